@@ -506,6 +506,102 @@ int s8kv_gather_slots(int num_tensors, void* const* tensor_ptrs, const int64_t* 
                       void* stream);
 
 /*
+ * Rotary positions of q and k (the role of superl8.rope and RotaryEmbedding
+ * before the cache write; the reference's rows are layers/rotary.py).
+ *
+ * q [num_tokens][num_q_heads][head_dim] and k [num_tokens][num_kv_heads][head_dim]
+ * at element strides, head_dim contiguous; k NULL with num_kv_heads 0: q alone.
+ * dtype: 0 fp16, 1 bf16, 2 fp32 (in and out).  Of each head the first rot_dim
+ * dims turn (even, <= head_dim), the others are copied.  pairing 0: dims p and
+ * p + rot_dim/2 are a pair, 1: dims 2p and 2p + 1.  cos_sin fp32
+ * [max_positions][rot_dim], contiguous: the cosines of a position's rot_dim/2
+ * pairs, then the sines.  positions int32 [num_axes][num_tokens], axes
+ * pos_axis_stride elements apart: one axis, or up to four (time, height,
+ * width, ..) with axis_map (host, uint64_t[4]) holding each pair's axis in two
+ * bits, pair p at bits 2 (p % 32) of word p / 32.  A position outside
+ * [0, max_positions) turns its pairs into NaN; nothing is read there.
+ * q_norm, k_norm: NULL, or [head_dim] weights (norm_dtype as dtype) of an RMS
+ * norm of each head before the rotation: x / sqrt(mean(x^2) + eps) * w.
+ * Arithmetic in fp32, one rounding at the end.  q_out may be q itself and
+ * k_out k itself (same pointer and strides); other overlaps are not allowed.
+ */
+int s8kv_rope(const void* q, int num_q_heads, int64_t q_stride_t, int64_t q_stride_h, const void* k,
+              int num_kv_heads, int64_t k_stride_t, int64_t k_stride_h, int64_t num_tokens, int head_dim, int dtype,
+              const int32_t* positions, int num_axes, int64_t pos_axis_stride, const uint64_t* axis_map,
+              const float* cos_sin, int64_t max_positions, int rot_dim, int pairing, const void* q_norm,
+              const void* k_norm, int norm_dtype, float eps, void* q_out, int64_t q_out_stride_t,
+              int64_t q_out_stride_h, void* k_out, int64_t k_out_stride_t, int64_t k_out_stride_h, void* stream);
+
+/*
+ * The append with the rotation on the way: s8kv_rope of q and k, then
+ * s8kv_append_int8 / s8kv_append_k8v3 of the rotated k and of v, in one
+ * launch.  q, k, v: fp16 or bf16 (dtype 0, 1); q_out and k_out are fp16 (the
+ * type the attention entry points take), k_out may be NULL.  The rotated k
+ * and v round to fp16 before they are quantized, so the cache bytes are those
+ * of the two calls.  Tokens with a negative slot, or one outside the pool,
+ * write no cache row; their q_out and k_out are written all the same.
+ */
+int s8kv_append_rope_int8(const void* q, int num_q_heads, int64_t q_stride_t, int64_t q_stride_h, const void* k,
+                          const void* v, int num_kv_heads, int64_t k_stride_t, int64_t k_stride_h,
+                          int64_t v_stride_t, int64_t v_stride_h, int64_t num_tokens, int head_dim, int dtype,
+                          const int32_t* positions, int num_axes, int64_t pos_axis_stride, const uint64_t* axis_map,
+                          const float* cos_sin, int64_t max_positions, int rot_dim, int pairing, const void* q_norm,
+                          const void* k_norm, int norm_dtype, float eps, void* q_out, int64_t q_out_stride_t,
+                          int64_t q_out_stride_h, void* k_out, int64_t k_out_stride_t, int64_t k_out_stride_h,
+                          const int32_t* slot_mapping, int8_t* k_cache, float* k_scale, int8_t* v_cache,
+                          float* v_scale, int64_t num_blocks, int block_size, void* stream);
+int s8kv_append_rope_k8v3(const void* q, int num_q_heads, int64_t q_stride_t, int64_t q_stride_h, const void* k,
+                          const void* v, int num_kv_heads, int64_t k_stride_t, int64_t k_stride_h,
+                          int64_t v_stride_t, int64_t v_stride_h, int64_t num_tokens, int head_dim, int dtype,
+                          const int32_t* positions, int num_axes, int64_t pos_axis_stride, const uint64_t* axis_map,
+                          const float* cos_sin, int64_t max_positions, int rot_dim, int pairing, const void* q_norm,
+                          const void* k_norm, int norm_dtype, float eps, void* q_out, int64_t q_out_stride_t,
+                          int64_t q_out_stride_h, void* k_out, int64_t k_out_stride_t, int64_t k_out_stride_h,
+                          const int32_t* slot_mapping, int8_t* k_cache, float* k_scale, int32_t* v_packed,
+                          float* v_norm, const float* v_codebook, int lloyd_block, int64_t num_blocks,
+                          int block_size, void* stream);
+
+/*
+ * Causal linear attention with one decay per head (the role of the
+ * reference's layers/linear_attn.py ops on hybrid models): per token
+ *   S <- exp(log_decay[h]) S + k_t v_t^T,   o_t = scale q_t^T S,
+ * S fp32 [head_dim][head_dim] (key dims by value dims) per sequence and query
+ * head, in a pool: slot s, head h at state + s state_stride_slot + h
+ * head_dim^2.  Query head h reads key / value head h / (num_q_heads /
+ * num_kv_heads).  q, k, v, out: fp16 or bf16 (dtype 0, 1) token-major rows at
+ * element strides, head_dim contiguous.  log_decay fp32 [num_q_heads], <= 0
+ * (0: no decay, -inf: no memory).  state_slots int32 [batch], NULL: sequence b
+ * has slot b; two sequences of a call must not share a slot.  A slot outside
+ * [0, num_slots) makes its sequence a padding row: zeros out, no state read or
+ * written.  reset uint8 [batch] or NULL: a non-zero entry starts its sequence
+ * from an empty state (the slot's old contents are not read), so a sequence
+ * of no tokens leaves zeros there.  A non-finite state or input makes the
+ * outputs that depend on it non-finite, and no other.
+ *
+ * _varlen: sequence b's tokens are [cu_seqlens[b], cu_seqlens[b + 1]) (device
+ * int32 [batch + 1]); max_seqlen only sizes the launch.  Rows of out behind
+ * the last sequence are zeros.  workspace: s8kv_linear_attn_workspace_size
+ * bytes (16-byte aligned, no initialisation) let long sequences be split
+ * across workgroups; NULL or a smaller one runs unsplit.  Calls that overlap
+ * on one workspace race.
+ * _decode: one token per sequence.
+ */
+int64_t s8kv_linear_attn_workspace_size(int batch, int num_q_heads, int head_dim, int max_seqlen);
+int s8kv_linear_attn_varlen(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k, int64_t k_stride_t,
+                            int64_t k_stride_h, const void* v, int64_t v_stride_t, int64_t v_stride_h,
+                            int64_t num_tokens, int num_q_heads, int num_kv_heads, int head_dim, int dtype,
+                            const float* log_decay, float* state, int64_t state_stride_slot, int64_t num_slots,
+                            const int32_t* state_slots, const uint8_t* reset, const int32_t* cu_seqlens, int batch,
+                            int max_seqlen, float scale, void* out, int64_t out_stride_t, int64_t out_stride_h,
+                            void* workspace, int64_t workspace_bytes, void* stream);
+int s8kv_linear_attn_decode(const void* q, int64_t q_stride_b, int64_t q_stride_h, const void* k, int64_t k_stride_b,
+                            int64_t k_stride_h, const void* v, int64_t v_stride_b, int64_t v_stride_h, int batch,
+                            int num_q_heads, int num_kv_heads, int head_dim, int dtype, const float* log_decay,
+                            float* state, int64_t state_stride_slot, int64_t num_slots, const int32_t* state_slots,
+                            const uint8_t* reset, float scale, void* out, int64_t out_stride_b, int64_t out_stride_h,
+                            void* stream);
+
+/*
  * Kernel timing (diagnostics; no counterpart in the reference).  Between
  * s8kv_timing_begin() and s8kv_timing_end(), every decode call made outside
  * graph capture launches its kernel with HIP events stamped with the

@@ -168,6 +168,34 @@ SIGNATURES: dict[str, tuple] = {
         _i32, ctypes.POINTER(_c_void_p), ctypes.POINTER(_i64), ctypes.POINTER(_i64), _i32, _i32, _i64, _i32,
         _c_void_p, _c_void_p, _i32, _c_void_p,
     ]),
+    "s8kv_rope": (_i32, [
+        _c_void_p, _i32, _i64, _i64, _c_void_p, _i32, _i64, _i64, _i64, _i32, _i32,
+        _c_void_p, _i32, _i64, _c_void_p, _c_void_p, _i64, _i32, _i32, _c_void_p, _c_void_p, _i32, _f32,
+        _c_void_p, _i64, _i64, _c_void_p, _i64, _i64, _c_void_p,
+    ]),
+    "s8kv_append_rope_int8": (_i32, [
+        _c_void_p, _i32, _i64, _i64, _c_void_p, _c_void_p, _i32, _i64, _i64, _i64, _i64, _i64, _i32, _i32,
+        _c_void_p, _i32, _i64, _c_void_p, _c_void_p, _i64, _i32, _i32, _c_void_p, _c_void_p, _i32, _f32,
+        _c_void_p, _i64, _i64, _c_void_p, _i64, _i64,
+        _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i32, _c_void_p,
+    ]),
+    "s8kv_append_rope_k8v3": (_i32, [
+        _c_void_p, _i32, _i64, _i64, _c_void_p, _c_void_p, _i32, _i64, _i64, _i64, _i64, _i64, _i32, _i32,
+        _c_void_p, _i32, _i64, _c_void_p, _c_void_p, _i64, _i32, _i32, _c_void_p, _c_void_p, _i32, _f32,
+        _c_void_p, _i64, _i64, _c_void_p, _i64, _i64,
+        _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i32, _i64, _i32, _c_void_p,
+    ]),
+    "s8kv_linear_attn_workspace_size": (_i64, [_i32, _i32, _i32, _i32]),
+    "s8kv_linear_attn_varlen": (_i32, [
+        _c_void_p, _i64, _i64, _c_void_p, _i64, _i64, _c_void_p, _i64, _i64, _i64, _i32, _i32, _i32, _i32,
+        _c_void_p, _c_void_p, _i64, _i64, _c_void_p, _c_void_p, _c_void_p, _i32, _i32, _f32,
+        _c_void_p, _i64, _i64, _c_void_p, _i64, _c_void_p,
+    ]),
+    "s8kv_linear_attn_decode": (_i32, [
+        _c_void_p, _i64, _i64, _c_void_p, _i64, _i64, _c_void_p, _i64, _i64, _i32, _i32, _i32, _i32, _i32,
+        _c_void_p, _c_void_p, _i64, _i64, _c_void_p, _c_void_p, _f32,
+        _c_void_p, _i64, _i64, _c_void_p,
+    ]),
     "s8kv_timing_begin": (_i32, []),
     "s8kv_timing_end": (_i32, [ctypes.POINTER(_i32), ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_double)]),
     "s8kv_probe_read_tiles": (_i32, [

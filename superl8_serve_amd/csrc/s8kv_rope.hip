@@ -1,0 +1,672 @@
+// Rotary positions of q and k, alone or on the way into the paged cache.
+//
+// A head of D values holds R / 2 pairs (R <= D, the other dims pass through):
+// (x_p, x_{p + R/2}) with half-split pairing, (x_2p, x_{2p+1}) with adjacent
+// pairing.  Pair p belongs to one position axis a(p) and turns by the angle of
+// that axis's position: c = table[pos_a][p], s = table[pos_a][R/2 + p],
+//   (x1, x2) -> (x1 c - x2 s, x2 c + x1 s),
+// two fp32 products and one fp32 add per value, each rounded by itself (no
+// contraction, so that the bytes do not hang on the compiler's choice).  With
+// a norm weight the head is first scaled to x r w, r = 1 / sqrt(mean(x^2) +
+// eps), in fp32 with the squares added by a pairwise tree.  The result is
+// rounded once, to the output's type; K rounds to fp16 and then goes the
+// append's way (Hadamard, fp16, RTN int8), so the cache holds the bytes that
+// the rotation followed by the append would store.
+#include "s8kv_append_rows.h"
+#include "s8kv_host.h"
+
+#pragma clang fp contract(off)
+
+namespace s8kv {
+namespace rope {
+
+constexpr int kWaves = 4;  // waves per workgroup
+
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+
+// element types: 0 fp16, 1 bf16, 2 fp32
+template <int DT>
+constexpr int kBytes = DT == 2 ? 4 : 2;
+
+__device__ __forceinline__ float pin(float x) {  // keeps the product's rounding apart from what follows
+  asm("" : "+v"(x));
+  return x;
+}
+
+__device__ __forceinline__ float load_any(const void* p, int64_t i, int dtype) {
+  if (dtype == 0) return (float)static_cast<const _Float16*>(p)[i];
+  if (dtype == 1) return __builtin_bit_cast(float, (uint32_t) static_cast<const uint16_t*>(p)[i] << 16);
+  return static_cast<const float*>(p)[i];
+}
+
+struct Rows {  // [tokens][heads][D], unit stride on D; strides in elements
+  char* p;
+  int64_t st, sh;
+  int heads;
+  const void* norm;  // [D] weight, or NULL
+};
+
+struct Args {
+  Rows q, k, v;
+  char *q_out, *k_out;  // k_out may be NULL in the writing modes
+  int64_t qo_t, qo_h, ko_t, ko_h;
+  int64_t tokens;
+  const int32_t* pos;  // [axes][tokens]
+  int64_t pos_stride;
+  int axes;
+  uint64_t axis_map[4];  // two bits per pair
+  const float* table;    // [max_pos][R]: cos of the R/2 pairs, then sin
+  int64_t max_pos;
+  int rot;
+  int adjacent;
+  int partner;  // half pairing: parts between a pair's values (1, 2, 4, 8), 0: both on one lane
+  int norm_dtype;
+  float eps, inv_d;
+  int hpi_log2;      // heads per iteration of a wave
+  int iters, per_wave;  // iterations over q, k and v heads; of them, a wave's
+  // writing modes
+  const int32_t* slot_mapping;
+  char *k_cache, *v_cache;
+  float *k_scale, *v_scale;
+  const float* v_codebook;
+  int64_t num_blocks;
+  int block_size_log2;
+  float rot_norm;
+};
+
+// The lane's 16 values of a row (or, fast path, four 16-byte words of it).
+template <int DT>
+struct Raw {
+  u32x4_t w[DT == 2 ? 4 : 2];
+};
+template <int DT>
+__device__ __forceinline__ Raw<DT> load_raw(const char* p) {
+  Raw<DT> r;
+#pragma unroll
+  for (int i = 0; i < (DT == 2 ? 4 : 2); ++i) r.w[i] = reinterpret_cast<const u32x4_t*>(p)[i];
+  return r;
+}
+template <int DT>
+__device__ __forceinline__ void expand(const Raw<DT>& r, float (&x)[16]) {
+  if constexpr (DT == 0) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const half8_t h = __builtin_bit_cast(half8_t, r.w[j]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[8 * j + i] = (float)h[i];
+    }
+  } else if constexpr (DT == 1) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t u = r.w[j / 4][j % 4];
+      x[2 * j] = __builtin_bit_cast(float, u << 16);
+      x[2 * j + 1] = __builtin_bit_cast(float, u & 0xFFFF0000u);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) x[j] = __builtin_bit_cast(float, (uint32_t)r.w[j / 4][j % 4]);
+  }
+}
+template <int DT>
+__device__ __forceinline__ void store_part(char* p, const float (&x)[16]) {
+  u32x4_t* o = reinterpret_cast<u32x4_t*>(p);
+  if constexpr (DT == 0) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      half8_t h;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) h[i] = (_Float16)pin(x[8 * j + i]);
+      o[j] = __builtin_bit_cast(u32x4_t, h);
+    }
+  } else if constexpr (DT == 1) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      bf16x8_t h;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) h[i] = (__bf16)pin(x[8 * j + i]);
+      o[j] = __builtin_bit_cast(u32x4_t, h);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      o[j] = u32x4_t{__builtin_bit_cast(uint32_t, x[4 * j]), __builtin_bit_cast(uint32_t, x[4 * j + 1]),
+                     __builtin_bit_cast(uint32_t, x[4 * j + 2]), __builtin_bit_cast(uint32_t, x[4 * j + 3])};
+  }
+}
+
+// The table row of pair p's axis: the address of (cos, pair 0), or NULL for a
+// position outside the table (its pairs become NaN; nothing is read).
+__device__ __forceinline__ const float* table_row(const Args& a, int pos) {
+  return pos >= 0 && (int64_t)pos < a.max_pos ? a.table + (int64_t)pos * a.rot : nullptr;
+}
+__device__ __forceinline__ int axis_of(const Args& a, int pair) {
+  const uint64_t m = pair < 64 ? (pair < 32 ? a.axis_map[0] : a.axis_map[1]) : (pair < 96 ? a.axis_map[2] : a.axis_map[3]);
+  return (int)(m >> (2 * (pair & 31))) & 3;
+}
+__device__ __forceinline__ int position(const Args& a, int axis, int64_t t) { return a.pos[axis * a.pos_stride + t]; }
+
+// cos and signed sin (-s for a pair's first value, +s for its second) of the
+// lane's 16 values; 1 and 0 are not used for the dims past R (`turns` false).
+template <int D>
+struct Angles {
+  float c[16], s[16];
+  bool turns;
+  __device__ __forceinline__ void load(const Args& a, int64_t t, bool live, int li) {
+    const int half = a.rot >> 1;
+    turns = 16 * li < a.rot;
+    const float nan = __builtin_nanf("");
+#pragma unroll
+    for (int i = 0; i < 16; ++i) c[i] = s[i] = nan;
+    if (!live || !turns) return;
+    if (a.axes == 1) {
+      const float* row = table_row(a, position(a, 0, t));
+      if (!row) return;
+      if (a.adjacent) {
+        const float4_t* cp = reinterpret_cast<const float4_t*>(row + 8 * li);
+        const float4_t* sp = reinterpret_cast<const float4_t*>(row + half + 8 * li);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float4_t cv = cp[j], sv = sp[j];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            c[8 * j + 2 * i] = c[8 * j + 2 * i + 1] = cv[i];
+            s[8 * j + 2 * i] = -sv[i];
+            s[8 * j + 2 * i + 1] = sv[i];
+          }
+        }
+      } else if (a.partner) {
+        const bool second = (li & a.partner) != 0;
+        const int p0 = 16 * (li & (a.partner - 1));
+        const float4_t* cp = reinterpret_cast<const float4_t*>(row + p0);
+        const float4_t* sp = reinterpret_cast<const float4_t*>(row + half + p0);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float4_t cv = cp[j], sv = sp[j];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            c[4 * j + i] = cv[i];
+            s[4 * j + i] = second ? sv[i] : -sv[i];
+          }
+        }
+      } else {  // R = 16: pairs (i, i + 8) of part 0
+        const float4_t* cp = reinterpret_cast<const float4_t*>(row);
+        const float4_t* sp = reinterpret_cast<const float4_t*>(row + 8);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float4_t cv = cp[j], sv = sp[j];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            c[4 * j + i] = c[8 + 4 * j + i] = cv[i];
+            s[4 * j + i] = -sv[i];
+            s[8 + 4 * j + i] = sv[i];
+          }
+        }
+      }
+      return;
+    }
+    // several axes: the pairs' rows differ
+    const float* rows[4];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) rows[x] = x < a.axes ? table_row(a, position(a, x, t)) : nullptr;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      int pair;
+      bool second;
+      if (a.adjacent) {
+        pair = 8 * li + i / 2;
+        second = i & 1;
+      } else if (a.partner) {
+        pair = 16 * (li & (a.partner - 1)) + i;
+        second = (li & a.partner) != 0;
+      } else {
+        pair = i & 7;
+        second = i >= 8;
+      }
+      const int ax = axis_of(a, pair);
+      const float* row = ax < 2 ? (ax == 0 ? rows[0] : rows[1]) : (ax == 2 ? rows[2] : rows[3]);
+      if (row) {
+        c[i] = row[pair];
+        const float sv = row[half + pair];
+        s[i] = second ? sv : -sv;
+      }
+    }
+  }
+  __device__ __forceinline__ void turn(const Args& a, float (&x)[16]) const {
+    float y[16];
+    if (a.adjacent) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) y[i] = x[i ^ 1];
+    } else if (a.partner == 1) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) y[i] = xor_partner<1>(x[i]);
+    } else if (a.partner == 2) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) y[i] = xor_partner<2>(x[i]);
+    } else if (a.partner == 4) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) y[i] = xor_partner<RowsLayout<D>::LANE4>(x[i]);
+    } else if (a.partner == 8) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) y[i] = xor_partner<8>(x[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) y[i] = x[i ^ 8];
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float r = x[i] * c[i] + y[i] * s[i];
+      x[i] = turns ? r : x[i];
+    }
+  }
+};
+
+// x -> x r w: the squares add up by a pairwise tree over neighbouring dims
+// (in-lane, then across the row's lanes), mean, + eps, correctly rounded
+// square root and reciprocal.
+template <int D>
+__device__ __forceinline__ void normalise(const Args& a, const void* weight, float (&x)[16], int li) {
+  constexpr int LPR = RowsLayout<D>::LPR;
+  float s[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) s[i] = x[i] * x[i];
+#pragma unroll
+  for (int h = 1; h < 16; h <<= 1) {
+#pragma unroll
+    for (int i = 0; i < 16; i += 2 * h) s[i] = s[i] + s[i + h];
+  }
+  float t = s[0];
+  if constexpr (LPR > 1) t = t + xor_partner<1>(t);
+  if constexpr (LPR > 2) t = t + xor_partner<2>(t);
+  if constexpr (LPR > 4) t = t + xor_partner<RowsLayout<D>::LANE4>(t);
+  if constexpr (LPR > 8) t = t + xor_partner<8>(t);
+  const float r = 1.0f / __builtin_sqrtf(t * a.inv_d + a.eps);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) x[i] = x[i] * r * load_any(weight, 16 * li + i, a.norm_dtype);
+}
+
+// A token's cache row of KV head h, or false: a negative slot or one outside
+// the pool writes nothing.
+__device__ __forceinline__ bool cache_row(const Args& a, int64_t t, int h, uint64_t& row) {
+  const int32_t slot = a.slot_mapping[t];
+  const uint32_t blk = (uint32_t)slot >> a.block_size_log2;
+  row = (((uint64_t)blk * (uint32_t)a.k.heads + (uint32_t)h) << a.block_size_log2) +
+        ((uint32_t)slot & ((1u << a.block_size_log2) - 1u));
+  return slot >= 0 && (int64_t)blk < a.num_blocks;
+}
+
+// modes: 0 q and k out, 1 int8 cache, 2 K8V3 cache
+template <int D, int DT, int MODE>
+__global__ __launch_bounds__(64 * kWaves) void rope_rows_kernel(Args a) {
+  using L = RowsLayout<D>;
+  const int lane = threadIdx.x & 63;
+  const int li = L::part(lane);
+  const int chunks = (a.iters + a.per_wave - 1) / a.per_wave;
+  const int64_t wave = (int64_t)blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int64_t group = wave / chunks;
+  const int it0 = (int)(wave - group * chunks) * a.per_wave;
+  const int it1 = min(a.iters, it0 + a.per_wave);
+  const int hpi = 1 << a.hpi_log2;
+  const int64_t t = group * (L::RPW >> a.hpi_log2) + (L::row(lane) >> a.hpi_log2);
+  const int sub = L::row(lane) & (hpi - 1);
+  const bool here = t < a.tokens;
+  const int nq = (a.q.heads + hpi - 1) >> a.hpi_log2, nk = (a.k.heads + hpi - 1) >> a.hpi_log2;
+
+  Angles<D> angles;
+  if (it0 < nq + nk) angles.load(a, t, here, li);
+  const RowsHadamard<D> hadamard(li, a.rot_norm);
+  float cb[8], thr[8];
+  if constexpr (MODE == 2) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) cb[i] = thr[i] = a.v_codebook[i];
+  }
+
+#pragma unroll 1
+  for (int it = it0; it < it1; ++it) {
+    const int kind = it < nq ? 0 : (it < nq + nk ? 1 : 2);
+    const Rows& rows = kind == 0 ? a.q : (kind == 1 ? a.k : a.v);
+    const int h = ((kind == 0 ? it : (kind == 1 ? it - nq : it - nq - nk)) << a.hpi_log2) + sub;
+    const bool live = here && h < rows.heads;
+    Raw<DT> raw{};
+    if (live) raw = load_raw<DT>(rows.p + (t * rows.st + h * rows.sh + 16 * li) * kBytes<DT>);
+    float x[16];
+    expand<DT>(raw, x);
+    if (kind < 2) {
+      if (rows.norm) normalise<D>(a, rows.norm, x, li);
+      angles.turn(a, x);
+      char* out = kind == 0 ? a.q_out : a.k_out;
+      if (live && out) {
+        const int64_t off = kind == 0 ? t * a.qo_t + h * a.qo_h : t * a.ko_t + h * a.ko_h;
+        constexpr int OT = MODE ? 0 : DT;  // the writing modes hand q and k on in fp16
+        store_part<OT>(out + (off + 16 * li) * kBytes<OT>, x);
+      }
+    }
+    if constexpr (MODE > 0) {
+      if (kind == 0) continue;
+      uint64_t row = 0;
+      const bool write = live && cache_row(a, t, h, row);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] = (float)(_Float16)pin(x[i]);
+      if (kind == 1) {
+        hadamard(x);
+        rows_rtn_store<D>(x, write, li, PtrOut{a.k_cache + row * D}, PtrOut{reinterpret_cast<char*>(a.k_scale + row)});
+      } else if constexpr (MODE == 1) {
+        rows_rtn_store<D>(x, write, li, PtrOut{a.v_cache + row * D}, PtrOut{reinterpret_cast<char*>(a.v_scale + row)});
+      } else {
+        rows_lloydmax3_store<D>(x, write, li, false, cb, thr, PtrOut{a.v_cache + row * (D / 32 * 3 * 4)},
+                                PtrOut{reinterpret_cast<char*>(a.v_scale + row * (D / 128))});
+      }
+    }
+  }
+}
+
+// Any alignment, any even R: one wave per row, lane l holds dims l, l + 64, ..
+// and reads its pairs' other values itself.  The arithmetic and its order are
+// the kernel's above.
+template <int D, int DT, int MODE>
+__global__ __launch_bounds__(64 * kWaves) void rope_kernel(Args a) {
+  constexpr int E = RowLayout<D>::E;
+  constexpr int OT = MODE ? 0 : DT;
+  const int lane = threadIdx.x & 63;
+  const bool active = lane < RowLayout<D>::ACTIVE;
+  const int heads = a.q.heads + a.k.heads + a.v.heads;
+  const int64_t id = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6);
+  if (id >= a.tokens * heads) return;
+  const int64_t t = id / heads;
+  int h = (int)(id - t * heads);
+  const int kind = h < a.q.heads ? 0 : (h < a.q.heads + a.k.heads ? 1 : 2);
+  const Rows& rows = kind == 0 ? a.q : (kind == 1 ? a.k : a.v);
+  h -= kind == 0 ? 0 : (kind == 1 ? a.q.heads : a.q.heads + a.k.heads);
+  const char* src = rows.p + (t * rows.st + h * rows.sh) * kBytes<DT>;
+  float x[E];
+#pragma unroll
+  for (int j = 0; j < E; ++j) x[j] = active ? load_any(src, lane + 64 * j, DT) : 0.0f;
+  if (kind < 2) {
+    const int half = a.rot >> 1;
+    float y[E], c[E], s[E];
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      const int d = lane + 64 * j;
+      y[j] = 0.0f;
+      c[j] = s[j] = __builtin_nanf("");
+      if (active && d < a.rot) {
+        const int pair = a.adjacent ? d >> 1 : (d < half ? d : d - half);
+        const bool second = a.adjacent ? d & 1 : d >= half;
+        y[j] = load_any(src, a.adjacent ? d ^ 1 : (second ? d - half : d + half), DT);
+        const float* row = table_row(a, position(a, a.axes == 1 ? 0 : axis_of(a, pair), t));
+        if (row) {
+          c[j] = row[pair];
+          s[j] = second ? row[half + pair] : -row[half + pair];
+        }
+      }
+    }
+    if (rows.norm) {
+      float sq[E];
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        sq[j] = x[j] * x[j];
+#pragma unroll
+        for (int m = 1; m <= 32; m <<= 1) {
+          if (m < D) sq[j] = sq[j] + shfl_xor_f(sq[j], m);
+        }
+      }
+#pragma unroll
+      for (int w = 1; w < E; w <<= 1) {
+#pragma unroll
+        for (int j = 0; j < E; j += 2 * w) sq[j] = sq[j] + sq[j + w];
+      }
+      const float r = 1.0f / __builtin_sqrtf(sq[0] * a.inv_d + a.eps);
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        const int d = lane + 64 * j;
+        if (active) {
+          x[j] = x[j] * r * load_any(rows.norm, d, a.norm_dtype);
+          if (d < a.rot)
+            y[j] = y[j] * r * load_any(rows.norm, a.adjacent ? d ^ 1 : (d < half ? d + half : d - half), a.norm_dtype);
+        }
+      }
+    }
+    char* out = kind == 0 ? a.q_out : a.k_out;
+    const int64_t off = kind == 0 ? t * a.qo_t + h * a.qo_h : t * a.ko_t + h * a.ko_h;
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      const int d = lane + 64 * j;
+      const float r = x[j] * c[j] + y[j] * s[j];
+      x[j] = d < a.rot ? r : x[j];
+      if (active && out) {
+        if constexpr (OT == 0) reinterpret_cast<_Float16*>(out)[off + d] = (_Float16)pin(x[j]);
+        else if constexpr (OT == 1) reinterpret_cast<__bf16*>(out)[off + d] = (__bf16)pin(x[j]);
+        else reinterpret_cast<float*>(out)[off + d] = x[j];
+      }
+    }
+  }
+  if constexpr (MODE > 0) {
+    uint64_t row = 0;
+    if (kind == 0 || !cache_row(a, t, h, row)) return;
+#pragma unroll
+    for (int j = 0; j < E; ++j) x[j] = (float)(_Float16)pin(x[j]);
+    if (kind == 1) {
+      fwht_row<D>(x, lane);
+#pragma unroll
+      for (int j = 0; j < E; ++j) x[j] = (float)(_Float16)materialize(x[j] * a.rot_norm);
+      rtn_store_row<D>(x, lane, PtrOut{a.k_cache + row * D}, PtrOut{reinterpret_cast<char*>(a.k_scale + row)});
+    } else if constexpr (MODE == 1) {
+      rtn_store_row<D>(x, lane, PtrOut{a.v_cache + row * D}, PtrOut{reinterpret_cast<char*>(a.v_scale + row)});
+    } else {
+      constexpr int NB = D / 128, WORDS = D / 32 * 3;
+      float cb[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) cb[i] = a.v_codebook[i];
+      uint32_t w;
+      float nv;
+      lloydmax3_encode_row<D>(x, cb, lane, w, nv);
+      if (lane < WORDS) PtrOut{a.v_cache + row * (WORDS * 4)}.st32(lane * 4u, w);
+      if (lane < NB) PtrOut{reinterpret_cast<char*>(a.v_scale + row * NB)}.st32(lane * 4u, __builtin_bit_cast(uint32_t, nv));
+    }
+  }
+}
+
+static bool aligned(const void* p, int64_t st, int64_t sh, int bytes) {
+  return (uintptr_t)p % 16 == 0 && st * bytes % 16 == 0 && sh * bytes % 16 == 0;
+}
+
+template <int D, int DT, int MODE>
+static int launch(Args& a, const char* what, hipStream_t stream) {
+  const int bytes = kBytes<DT>, obytes = MODE ? 2 : bytes;
+  const int parts = a.rot / 32;  // half pairing: parts between a pair's values
+  const bool rows = aligned(a.q.p, a.q.st, a.q.sh, bytes) && aligned(a.k.p, a.k.st, a.k.sh, bytes) &&
+                    aligned(a.v.p, a.v.st, a.v.sh, bytes) && aligned(a.q_out, a.qo_t, a.qo_h, obytes) &&
+                    aligned(a.k_out, a.ko_t, a.ko_h, obytes) && (uintptr_t)a.table % 16 == 0 && a.rot % 16 == 0 &&
+                    (a.adjacent || a.rot == 16 || (a.rot % 32 == 0 && is_pow2(parts)));
+  if (rows) {
+    constexpr int RPW = RowsLayout<D>::RPW;
+    a.partner = a.adjacent || a.rot == 16 ? 0 : parts;
+    int fewest = a.q.heads;
+    if (a.k.heads && a.k.heads < fewest) fewest = a.k.heads;
+    a.hpi_log2 = 0;
+    while ((2 << a.hpi_log2) <= RPW && (2 << a.hpi_log2) <= fewest) ++a.hpi_log2;
+    const int hpi = 1 << a.hpi_log2, tokens = RPW >> a.hpi_log2;
+    a.iters = (a.q.heads + hpi - 1) / hpi + (a.k.heads + hpi - 1) / hpi + (a.v.heads + hpi - 1) / hpi;
+    const int64_t groups = (a.tokens + tokens - 1) / tokens;
+    const int64_t want = (int64_t)device_cus() * 4 * 8;  // waves that the GPU holds
+    const int64_t each = groups * a.iters / want;
+    a.per_wave = (int)(each < 1 ? 1 : (each > a.iters ? a.iters : each));
+    const int64_t waves = groups * ((a.iters + a.per_wave - 1) / a.per_wave);
+    const int64_t grid = (waves + kWaves - 1) / kWaves;
+    S8KV_REQUIRE(grid < (int64_t(1) << 31), S8KV_ERR_INVALID, "%s: too many tokens (%lld)", what, (long long)a.tokens);
+    hipLaunchKernelGGL((rope_rows_kernel<D, DT, MODE>), dim3((unsigned)grid), dim3(64 * kWaves), 0, stream, a);
+  } else {
+    const int64_t n = a.tokens * (a.q.heads + a.k.heads + a.v.heads);
+    const int64_t grid = (n + kWaves - 1) / kWaves;
+    S8KV_REQUIRE(grid < (int64_t(1) << 31), S8KV_ERR_INVALID, "%s: too many rows (%lld)", what, (long long)n);
+    hipLaunchKernelGGL((rope_kernel<D, DT, MODE>), dim3((unsigned)grid), dim3(64 * kWaves), 0, stream, a);
+  }
+  return check_launch(what);
+}
+
+template <int D, int MODE>
+static int launch_dtype(Args& a, int dtype, const char* what, hipStream_t stream) {
+  if (dtype == 0) return launch<D, 0, MODE>(a, what, stream);
+  if (dtype == 1) return launch<D, 1, MODE>(a, what, stream);
+  if constexpr (MODE == 0) return launch<D, 2, MODE>(a, what, stream);
+  return S8KV_ERR_UNSUPPORTED;
+}
+
+template <int MODE>
+static int launch_dim(Args& a, int head_dim, int dtype, const char* what, hipStream_t stream) {
+  switch (head_dim) {
+    case 32:
+      if constexpr (MODE < 2) return launch_dtype<32, MODE>(a, dtype, what, stream);
+      break;
+    case 64:
+      if constexpr (MODE < 2) return launch_dtype<64, MODE>(a, dtype, what, stream);
+      break;
+    case 128: return launch_dtype<128, MODE>(a, dtype, what, stream);
+    case 256: return launch_dtype<256, MODE>(a, dtype, what, stream);
+  }
+  return S8KV_ERR_UNSUPPORTED;
+}
+
+// What the rotation alone and the writing forms share.
+static int fill(Args& a, const char* what, const void* q, int num_q_heads, int64_t q_st, int64_t q_sh, const void* k,
+                int num_kv_heads, int64_t k_st, int64_t k_sh, int64_t num_tokens, int head_dim, int dtype,
+                const int32_t* positions, int num_axes, int64_t pos_axis_stride, const uint64_t* axis_map,
+                const float* cos_sin, int64_t max_positions, int rot_dim, int pairing, const void* q_norm,
+                const void* k_norm, int norm_dtype, float eps, void* q_out, int64_t qo_st, int64_t qo_sh, void* k_out,
+                int64_t ko_st, int64_t ko_sh) {
+  S8KV_REQUIRE(num_tokens >= 0 && num_q_heads > 0 && num_kv_heads >= 0, S8KV_ERR_INVALID,
+               "%s: %lld tokens, %d q heads, %d kv heads", what, (long long)num_tokens, num_q_heads, num_kv_heads);
+  S8KV_REQUIRE(head_dim_ok(head_dim), S8KV_ERR_UNSUPPORTED, "%s: head_dim %d not in {32,64,128,256}", what, head_dim);
+  S8KV_REQUIRE(dtype >= 0 && dtype <= 2 && norm_dtype >= 0 && norm_dtype <= 2, S8KV_ERR_INVALID, "%s: unknown dtype", what);
+  S8KV_REQUIRE(rot_dim > 0 && rot_dim % 2 == 0 && rot_dim <= head_dim, S8KV_ERR_INVALID,
+               "%s: rot_dim %d must be even and in [2, head_dim %d]", what, rot_dim, head_dim);
+  S8KV_REQUIRE(pairing == 0 || pairing == 1, S8KV_ERR_INVALID, "%s: pairing %d not in {0, 1}", what, pairing);
+  S8KV_REQUIRE(num_axes >= 1 && num_axes <= 4 && (num_axes == 1 || axis_map), S8KV_ERR_INVALID,
+               "%s: %d position axes (1 to 4, with an axis map for more than one)", what, num_axes);
+  if (num_axes > 1)
+    for (int p = 0; p < rot_dim / 2; ++p)
+      S8KV_REQUIRE((int)((axis_map[p / 32] >> (2 * (p % 32))) & 3) < num_axes, S8KV_ERR_INVALID,
+                   "%s: pair %d is on an axis past %d", what, p, num_axes);
+  S8KV_REQUIRE(max_positions > 0, S8KV_ERR_INVALID, "%s: an empty cos / sin table", what);
+  S8KV_REQUIRE(num_tokens == 0 || (q && q_out && positions && cos_sin && (num_kv_heads == 0 || k)), S8KV_ERR_INVALID,
+               "%s: null pointer", what);
+  a.q = Rows{(char*)q, q_st, q_sh, num_q_heads, q_norm};
+  a.k = Rows{(char*)k, k_st, k_sh, num_kv_heads, k_norm};
+  a.q_out = (char*)q_out;
+  a.k_out = (char*)k_out;
+  a.qo_t = qo_st; a.qo_h = qo_sh;
+  a.ko_t = ko_st; a.ko_h = ko_sh;
+  a.tokens = num_tokens;
+  a.pos = positions;
+  a.pos_stride = pos_axis_stride;
+  a.axes = num_axes;
+  if (num_axes > 1)
+    for (int i = 0; i < 4; ++i) a.axis_map[i] = axis_map[i];
+  a.table = cos_sin;
+  a.max_pos = max_positions;
+  a.rot = rot_dim;
+  a.adjacent = pairing;
+  a.norm_dtype = norm_dtype;
+  a.eps = eps;
+  a.inv_d = 1.0f / (float)head_dim;
+  a.rot_norm = (float)(1.0 / __builtin_sqrt((double)head_dim));
+  return S8KV_OK;
+}
+
+static int fill_cache(Args& a, const char* what, const void* v, int64_t v_st, int64_t v_sh, const int32_t* slot_mapping,
+                      void* k_cache, float* k_scale, void* v_cache, float* v_scale, int64_t num_blocks,
+                      int block_size) {
+  S8KV_REQUIRE(a.k.heads > 0, S8KV_ERR_INVALID, "%s: num_kv_heads must be > 0", what);
+  S8KV_REQUIRE(is_pow2(block_size) && block_size >= 4, S8KV_ERR_UNSUPPORTED,
+               "%s: block_size %d must be a power of two >= 4", what, block_size);
+  S8KV_REQUIRE(num_blocks > 0, S8KV_ERR_INVALID, "%s: num_blocks must be > 0", what);
+  S8KV_REQUIRE(fits_u32(num_blocks * a.k.heads * block_size), S8KV_ERR_UNSUPPORTED,
+               "%s: more than 2^32 cache rows per layer", what);
+  S8KV_REQUIRE(a.tokens == 0 || (v && slot_mapping), S8KV_ERR_INVALID, "%s: null pointer", what);
+  S8KV_REQUIRE(k_cache && k_scale && v_cache && v_scale, S8KV_ERR_INVALID, "%s: null cache pointer", what);
+  a.v = Rows{(char*)v, v_st, v_sh, a.k.heads, nullptr};
+  a.slot_mapping = slot_mapping;
+  a.k_cache = (char*)k_cache;
+  a.v_cache = (char*)v_cache;
+  a.k_scale = k_scale;
+  a.v_scale = v_scale;
+  a.num_blocks = num_blocks;
+  a.block_size_log2 = log2i(block_size);
+  return S8KV_OK;
+}
+
+}  // namespace rope
+}  // namespace s8kv
+
+using namespace s8kv;
+
+extern "C" int s8kv_rope(const void* q, int num_q_heads, int64_t q_stride_t, int64_t q_stride_h, const void* k,
+                         int num_kv_heads, int64_t k_stride_t, int64_t k_stride_h, int64_t num_tokens, int head_dim,
+                         int dtype, const int32_t* positions, int num_axes, int64_t pos_axis_stride,
+                         const uint64_t* axis_map, const float* cos_sin, int64_t max_positions, int rot_dim,
+                         int pairing, const void* q_norm, const void* k_norm, int norm_dtype, float eps, void* q_out,
+                         int64_t q_out_stride_t, int64_t q_out_stride_h, void* k_out, int64_t k_out_stride_t,
+                         int64_t k_out_stride_h, void* stream) {
+  rope::Args a{};
+  const char* what = "s8kv_rope";
+  if (int rc = rope::fill(a, what, q, num_q_heads, q_stride_t, q_stride_h, k, num_kv_heads, k_stride_t, k_stride_h,
+                          num_tokens, head_dim, dtype, positions, num_axes, pos_axis_stride, axis_map, cos_sin,
+                          max_positions, rot_dim, pairing, q_norm, k_norm, norm_dtype, eps, q_out, q_out_stride_t,
+                          q_out_stride_h, k_out, k_out_stride_t, k_out_stride_h))
+    return rc;
+  S8KV_REQUIRE(num_tokens == 0 || num_kv_heads == 0 || k_out, S8KV_ERR_INVALID, "%s: null pointer", what);
+  if (num_tokens == 0) return S8KV_OK;
+  return rope::launch_dim<0>(a, head_dim, dtype, what, (hipStream_t)stream);
+}
+
+extern "C" int s8kv_append_rope_int8(
+    const void* q, int num_q_heads, int64_t q_stride_t, int64_t q_stride_h, const void* k, const void* v,
+    int num_kv_heads, int64_t k_stride_t, int64_t k_stride_h, int64_t v_stride_t, int64_t v_stride_h,
+    int64_t num_tokens, int head_dim, int dtype, const int32_t* positions, int num_axes, int64_t pos_axis_stride,
+    const uint64_t* axis_map, const float* cos_sin, int64_t max_positions, int rot_dim, int pairing,
+    const void* q_norm, const void* k_norm, int norm_dtype, float eps, void* q_out, int64_t q_out_stride_t,
+    int64_t q_out_stride_h, void* k_out, int64_t k_out_stride_t, int64_t k_out_stride_h, const int32_t* slot_mapping,
+    int8_t* k_cache, float* k_scale, int8_t* v_cache, float* v_scale, int64_t num_blocks, int block_size,
+    void* stream) {
+  rope::Args a{};
+  const char* what = "s8kv_append_rope_int8";
+  S8KV_REQUIRE(dtype == 0 || dtype == 1, S8KV_ERR_INVALID, "%s: dtype must be fp16 or bf16", what);
+  if (int rc = rope::fill(a, what, q, num_q_heads, q_stride_t, q_stride_h, k, num_kv_heads, k_stride_t, k_stride_h,
+                          num_tokens, head_dim, dtype, positions, num_axes, pos_axis_stride, axis_map, cos_sin,
+                          max_positions, rot_dim, pairing, q_norm, k_norm, norm_dtype, eps, q_out, q_out_stride_t,
+                          q_out_stride_h, k_out, k_out_stride_t, k_out_stride_h))
+    return rc;
+  if (int rc = rope::fill_cache(a, what, v, v_stride_t, v_stride_h, slot_mapping, k_cache, k_scale, v_cache, v_scale,
+                                num_blocks, block_size))
+    return rc;
+  if (num_tokens == 0) return S8KV_OK;
+  return rope::launch_dim<1>(a, head_dim, dtype, what, (hipStream_t)stream);
+}
+
+extern "C" int s8kv_append_rope_k8v3(
+    const void* q, int num_q_heads, int64_t q_stride_t, int64_t q_stride_h, const void* k, const void* v,
+    int num_kv_heads, int64_t k_stride_t, int64_t k_stride_h, int64_t v_stride_t, int64_t v_stride_h,
+    int64_t num_tokens, int head_dim, int dtype, const int32_t* positions, int num_axes, int64_t pos_axis_stride,
+    const uint64_t* axis_map, const float* cos_sin, int64_t max_positions, int rot_dim, int pairing,
+    const void* q_norm, const void* k_norm, int norm_dtype, float eps, void* q_out, int64_t q_out_stride_t,
+    int64_t q_out_stride_h, void* k_out, int64_t k_out_stride_t, int64_t k_out_stride_h, const int32_t* slot_mapping,
+    int8_t* k_cache, float* k_scale, int32_t* v_packed, float* v_norm, const float* v_codebook, int lloyd_block,
+    int64_t num_blocks, int block_size, void* stream) {
+  rope::Args a{};
+  const char* what = "s8kv_append_rope_k8v3";
+  S8KV_REQUIRE(dtype == 0 || dtype == 1, S8KV_ERR_INVALID, "%s: dtype must be fp16 or bf16", what);
+  if (int rc = rope::fill(a, what, q, num_q_heads, q_stride_t, q_stride_h, k, num_kv_heads, k_stride_t, k_stride_h,
+                          num_tokens, head_dim, dtype, positions, num_axes, pos_axis_stride, axis_map, cos_sin,
+                          max_positions, rot_dim, pairing, q_norm, k_norm, norm_dtype, eps, q_out, q_out_stride_t,
+                          q_out_stride_h, k_out, k_out_stride_t, k_out_stride_h))
+    return rc;
+  S8KV_REQUIRE(head_dim == 128 || head_dim == 256, S8KV_ERR_UNSUPPORTED, "%s: head_dim %d not in {128, 256}", what,
+               head_dim);
+  S8KV_REQUIRE(lloyd_block == 128, S8KV_ERR_UNSUPPORTED, "%s: lloyd_block %d != 128", what, lloyd_block);
+  S8KV_REQUIRE(v_codebook, S8KV_ERR_INVALID, "%s: null cache pointer", what);
+  if (int rc = rope::fill_cache(a, what, v, v_stride_t, v_stride_h, slot_mapping, k_cache, k_scale, v_packed, v_norm,
+                                num_blocks, block_size))
+    return rc;
+  a.v_codebook = v_codebook;
+  if (num_tokens == 0) return S8KV_OK;
+  return rope::launch_dim<2>(a, head_dim, dtype, what, (hipStream_t)stream);
+}

@@ -12,6 +12,7 @@ CPU tensors are rejected: there is no host implementation.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from collections.abc import Sequence
 
@@ -42,6 +43,11 @@ __all__ = [
     "snapkv_scores",
     "snapkv_scores_paged",
     "gather_slots",
+    "rope",
+    "quantize_kv_write_paged_rope",
+    "quantize_kv_write_paged_k8v3_rope",
+    "linear_attn_varlen",
+    "linear_attn_decode",
 ]
 
 
@@ -958,3 +964,304 @@ def gather_slots(tensors: Sequence[torch.Tensor], src_slots: Sequence[int], dst_
                                        (ctypes.c_int64 * n)(*lstrides), nl, hkv, nb, bs, src_t.data_ptr(),
                                        dst_t.data_ptr(), len(src_l), _stream(t0))
     _lib.check(rc, "gather_slots")
+
+
+# ---------------------------------------------------------------------------
+# Rotary positions, alone and on the way into the cache
+# ---------------------------------------------------------------------------
+
+
+def _launch(device: torch.device, entry, *args) -> int:
+    """``entry(*args)`` with ``device`` current: a launch on the default stream
+    (handle 0) goes to the current device, whatever the tensors' is."""
+    if device.index == torch._C._cuda_getDevice():
+        return entry(*args)
+    with torch.cuda.device(device):
+        return entry(*args)
+
+
+def _heads_view(x: torch.Tensor, name: str, tokens: int, dtype, dev) -> torch.Tensor:
+    """``x`` ``[tokens, heads, D]`` with a unit stride on D (copied if not)."""
+    _on_gpu(name, x, dtype, dev)
+    _require(x.dim() == 3 and x.shape[0] == tokens,
+             lambda: f"{name} must be [{tokens}, heads, head_dim], got {tuple(x.shape)}")
+    return x if x.stride(2) == 1 else x.contiguous()
+
+
+@functools.lru_cache(maxsize=256)
+def _axis_map(sections: tuple, interleaved: bool, half: int):
+    """The pairs' axes as the C ABI takes them, two bits a pair in four words."""
+    _require(2 <= len(sections) <= 4 and all(n >= 0 for n in sections) and sum(sections) == half,
+             lambda: f"sections {sections} must give 2 to 4 axes their share of the {half} pairs")
+    n = len(sections)
+    if interleaved:
+        _require(all(sections[a] == 0 or n * (sections[a] - 1) + a < half for a in range(1, n)),
+                 lambda: f"interleaved sections {sections} do not fit {half} pairs")
+        axes = [p % n if p < n * sections[p % n] else 0 for p in range(half)]
+    else:
+        axes = [a for a in range(n) for _ in range(sections[a])]
+    words = [0, 0, 0, 0]
+    for p, a in enumerate(axes):
+        words[p // 32] |= a << (2 * (p % 32))
+    return (ctypes.c_uint64 * 4)(*words)
+
+
+_PAIRINGS = {"half": 0, "adjacent": 1}
+
+
+def _rope_args(q, k, positions, cos_sin, sections, interleaved, pairing, q_norm, k_norm, eps):
+    """The checks and the C arguments that the rotation and the rotating
+    writes share: (tokens, rotation arguments, what must outlive the call)."""
+    dev, t, d = q.device, q.shape[0], q.shape[2]
+    _require(k is None or k.shape[2] == d, lambda: f"k head_dim {k.shape[2]} != q head_dim {d}")
+    _on_gpu("positions", positions, torch.int32, dev)
+    _on_gpu("cos_sin", cos_sin, torch.float32, dev)
+    _require(cos_sin.dim() == 2 and cos_sin.is_contiguous() and cos_sin.shape[0] > 0,
+             "cos_sin must be a contiguous [max_positions, rot_dim] tensor")
+    rot = cos_sin.shape[1]
+    _require(0 < rot <= d and rot % 2 == 0, lambda: f"cos_sin's rot_dim {rot} must be even and at most head_dim {d}")
+    if pairing not in _PAIRINGS:
+        raise ValueError(f"pairing must be 'half' or 'adjacent', got {pairing!r}")
+    if sections is None:
+        _require(not interleaved, "interleaved needs sections")
+        _require(tuple(positions.shape) in ((t,), (1, t)), lambda: f"positions must be [{t}], got {tuple(positions.shape)}")
+        axes, amap = 1, None
+    else:
+        amap = _axis_map(tuple(sections), bool(interleaved), rot // 2)
+        axes = len(sections)
+        _require(tuple(positions.shape) == (axes, t),
+                 lambda: f"positions must be [{axes}, {t}], got {tuple(positions.shape)}")
+    if t and positions.stride(-1) != 1:
+        positions = positions.contiguous()
+    norm_dtype = 0
+    norms = [None, None]
+    for i, (name, w) in enumerate((("q_norm", q_norm), ("k_norm", k_norm))):
+        if w is None:
+            continue
+        _on_gpu(name, w, None, dev)
+        _require(w.dtype in _ROT_DTYPES, lambda: f"{name}: dtype {w.dtype} not in fp16 / bf16 / fp32", TypeError)
+        _require(w.dim() == 1 and w.shape[0] == d, lambda: f"{name} must be [{d}], got {tuple(w.shape)}")
+        norms[i] = w if w.is_contiguous() else w.contiguous()
+        norm_dtype = _ROT_DTYPES[w.dtype]
+    _require(norms[0] is None or norms[1] is None or norms[0].dtype == norms[1].dtype, "q_norm and k_norm differ in dtype")
+    args = (positions.data_ptr(), axes, positions.stride(0) if positions.dim() == 2 else 0, amap, cos_sin.data_ptr(),
+            cos_sin.shape[0], rot, _PAIRINGS[pairing], None if norms[0] is None else norms[0].data_ptr(),
+            None if norms[1] is None else norms[1].data_ptr(), norm_dtype, eps)
+    return args, (positions, norms)
+
+
+def _rope_out(out, name: str, like: torch.Tensor, dtype) -> torch.Tensor:
+    if out is None:
+        return torch.empty(like.shape, dtype=dtype, device=like.device)
+    _on_gpu(name, out, dtype, like.device)
+    _require(out.shape == like.shape and out.stride(2) == 1,
+             lambda: f"{name} must be {tuple(like.shape)} with a unit stride on its last dim")
+    return out
+
+
+def rope(q, k, positions, cos_sin, *, sections=None, interleaved: bool = False, pairing: str = "half", q_norm=None,
+         k_norm=None, eps: float = 1e-6, q_out=None, k_out=None):
+    """Rotary positions of ``q`` ``[T, Hq, D]`` and ``k`` ``[T, Hkv, D]`` (or
+    None), fp16, bf16 or fp32, before the cache write or the prefill attention.
+
+    ``cos_sin``: fp32 ``[max_positions, R]``, the cosines of a position's R/2
+    pairs and then their sines (any frequency scaling is the table's); dims
+    past R are copied.  ``pairing``: "half" (dims p and p + R/2 are a pair) or
+    "adjacent" (2p and 2p + 1).  ``positions``: int32 ``[T]``, or ``[A, T]``
+    with ``sections``, the number of pairs of each of 2 to 4 axes (time,
+    height, width, ..): consecutive runs of pairs, or with ``interleaved`` the
+    pairs a, a + A, a + 2A, .. of each axis a > 0 and the others of axis 0.  A
+    position outside the table gives NaN.  ``q_norm`` / ``k_norm``: weights
+    ``[D]`` of an RMS norm of each head (``eps``) before the rotation.
+
+    fp32 arithmetic, one rounding.  Returns ``(q_out, k_out)``, new tensors or
+    the ones passed (``q`` / ``k`` themselves rotate in place)."""
+    _on_gpu("q", q)
+    _require(q.dtype in _ROT_DTYPES, lambda: f"rope: dtype {q.dtype} not in fp16 / bf16 / fp32", TypeError)
+    dev, dtype = q.device, q.dtype
+    _require(q.dim() == 3, lambda: f"q must be [tokens, heads, head_dim], got {tuple(q.shape)}")
+    t, hq, d = q.shape
+    src_q, src_k = _heads_view(q, "q", t, dtype, dev), None
+    if k is not None:
+        src_k = _heads_view(k, "k", t, dtype, dev)
+    args, keep = _rope_args(src_q, src_k, positions, cos_sin, sections, interleaved, pairing, q_norm, k_norm, eps)
+    q_out = _rope_out(q_out, "q_out", q, dtype)
+    if k is None:
+        _require(k_out is None, "k_out without k")
+        ks = (None, 0, 0, 0)
+        kos = (None, 0, 0)
+    else:
+        k_out = _rope_out(k_out, "k_out", k, dtype)
+        ks = (src_k.data_ptr(), k.shape[1], src_k.stride(0), src_k.stride(1))
+        kos = (k_out.data_ptr(), k_out.stride(0), k_out.stride(1))
+    if t and hq:
+        rc = _launch(dev, _lib.load().s8kv_rope, src_q.data_ptr(), hq, src_q.stride(0), src_q.stride(1), *ks, t, d,
+                     _ROT_DTYPES[dtype], *args, q_out.data_ptr(), q_out.stride(0), q_out.stride(1), *kos, _stream(q))
+        _lib.check(rc, "rope")
+    return q_out, k_out
+
+
+def _rope_write(what, entry, q, k, v, positions, cos_sin, k_cache, k_scale, slot_mapping, tail, sections, interleaved,
+                pairing, q_norm, k_norm, eps, q_out, k_out):
+    _require(q.dtype in (torch.float16, torch.bfloat16), lambda: f"{what}: dtype {q.dtype} not in fp16 / bf16", TypeError)
+    dev, dtype = q.device, q.dtype
+    _on_gpu("k_scale", k_scale, torch.float32, dev)
+    _on_gpu("slot_mapping", slot_mapping, torch.int32, dev)
+    n, hkv, bs, d = _cache_geometry(k_cache)
+    _require(tuple(k_scale.shape) == (n, hkv, bs) and k_scale.is_contiguous(), "k_scale must be [N, Hkv, bs] contiguous")
+    _require(q.dim() == 3 and q.shape[2] == d, lambda: f"q must be [tokens, heads, {d}], got {tuple(q.shape)}")
+    t, hq, _ = q.shape
+    src_q = _heads_view(q, "q", t, dtype, dev)
+    k, v = _heads_view(k, "k", t, dtype, dev), _heads_view(v, "v", t, dtype, dev)
+    _require(k.shape[1:] == (hkv, d) and v.shape == k.shape, lambda: f"k and v must be [{t}, {hkv}, {d}]")
+    _require(slot_mapping.dim() == 1 and slot_mapping.shape[0] == t, lambda: f"slot_mapping must be [{t}]")
+    slot_mapping = slot_mapping.contiguous()
+    args, keep = _rope_args(src_q, k, positions, cos_sin, sections, interleaved, pairing, q_norm, k_norm, eps)
+    q_out = _rope_out(q_out, "q_out", q, torch.float16)
+    if k_out is None:
+        kos = (None, 0, 0)
+    else:
+        k_out = _rope_out(k_out, "k_out", k, torch.float16)
+        kos = (k_out.data_ptr(), k_out.stride(0), k_out.stride(1))
+    if t and hq:
+        rc = _launch(dev, entry, src_q.data_ptr(), hq, src_q.stride(0), src_q.stride(1), k.data_ptr(), v.data_ptr(), hkv,
+                     k.stride(0), k.stride(1), v.stride(0), v.stride(1), t, d, _ROT_DTYPES[dtype], *args,
+                     q_out.data_ptr(), q_out.stride(0), q_out.stride(1), *kos, slot_mapping.data_ptr(),
+                     k_cache.data_ptr(), k_scale.data_ptr(), *tail, n, bs, _stream(q))
+        _lib.check(rc, what)
+    return q_out
+
+
+def quantize_kv_write_paged_rope(q, k, v, positions, cos_sin, k_cache, k_scale, v_cache, v_scale, slot_mapping, *,
+                                 sections=None, interleaved: bool = False, pairing: str = "half", q_norm=None,
+                                 k_norm=None, eps: float = 1e-6, q_out=None, k_out=None):
+    """``rope`` of ``q`` and ``k``, then ``quantize_kv_write_paged`` of the
+    rotated ``k`` and of ``v``, in one launch; the cache bytes are those of the
+    two calls.  ``q`` ``[T, Hq, D]``, ``k``, ``v`` ``[T, Hkv, D]``: fp16 or
+    bf16 (bf16 rows round to fp16 after the rotation, as the cache takes them).
+    Returns the rotated q in fp16 (``q_out``), what the decode and verify ops
+    take; ``k_out``: an fp16 tensor for the rotated k too (``attn_varlen`` over
+    fresh keys).  Tokens with a negative slot write no cache row.  The other
+    arguments are ``rope``'s."""
+    _on_gpu("q", q)
+    _on_gpu("k_cache", k_cache, torch.int8, q.device)
+    _on_gpu("v_cache", v_cache, torch.int8, q.device)
+    _on_gpu("v_scale", v_scale, torch.float32, q.device)
+    _require(v_cache.shape == k_cache.shape and v_cache.is_contiguous(), "v_cache must match k_cache")
+    _require(v_scale.shape == k_scale.shape and v_scale.is_contiguous(), "v_scale must be [N, Hkv, bs] contiguous")
+    return _rope_write("quantize_kv_write_paged_rope", _lib.load().s8kv_append_rope_int8, q, k, v, positions, cos_sin,
+                       k_cache, k_scale, slot_mapping, (v_cache.data_ptr(), v_scale.data_ptr()), sections, interleaved,
+                       pairing, q_norm, k_norm, eps, q_out, k_out)
+
+
+def quantize_kv_write_paged_k8v3_rope(q, k, v, positions, cos_sin, k_cache, k_scale, v_packed, v_norm, v_codebook,
+                                      slot_mapping, lloyd_block: int = 128, *, sections=None, interleaved: bool = False,
+                                      pairing: str = "half", q_norm=None, k_norm=None, eps: float = 1e-6, q_out=None,
+                                      k_out=None):
+    """``quantize_kv_write_paged_rope`` into the K8V3 layout (V as
+    ``quantize_kv_write_paged_k8v3`` writes it)."""
+    _on_gpu("q", q)
+    dev = q.device
+    _on_gpu("k_cache", k_cache, torch.int8, dev)
+    _on_gpu("v_packed", v_packed, torch.int32, dev)
+    _on_gpu("v_norm", v_norm, torch.float32, dev)
+    _on_gpu("v_codebook", v_codebook, torch.float32, dev)
+    n, hkv, bs, d = _cache_geometry(k_cache)
+    _require(lloyd_block == 128, lambda: f"lloyd_block {lloyd_block} != 128", RuntimeError)
+    _require(tuple(v_packed.shape) == (n, hkv, bs, d * 3 // 32) and v_packed.is_contiguous(),
+             "v_packed must be [N, Hkv, bs, D*3/32] contiguous")
+    _require(tuple(v_norm.shape) == (n, hkv, bs, d // lloyd_block) and v_norm.is_contiguous(),
+             "v_norm must be [N, Hkv, bs, D/lloyd_block] contiguous")
+    _require(v_codebook.numel() == 8 and v_codebook.is_contiguous(), "v_codebook must hold 8 contiguous entries")
+    return _rope_write("quantize_kv_write_paged_k8v3_rope", _lib.load().s8kv_append_rope_k8v3, q, k, v, positions,
+                       cos_sin, k_cache, k_scale, slot_mapping,
+                       (v_packed.data_ptr(), v_norm.data_ptr(), v_codebook.data_ptr(), lloyd_block), sections,
+                       interleaved, pairing, q_norm, k_norm, eps, q_out, k_out)
+
+
+# ---------------------------------------------------------------------------
+# Linear attention with a decay per head
+# ---------------------------------------------------------------------------
+
+
+def _linear_args(q, k, v, log_decay, state, state_slots, reset, batch):
+    """Checks shared by the two forms: (q, k, v, dtype code, what follows the
+    dtype in the C arguments, tensors that must outlive the call)."""
+    _on_gpu("q", q)
+    dev, dtype = q.device, q.dtype
+    _require(dtype in (torch.float16, torch.bfloat16), lambda: f"linear_attn: dtype {dtype} not in fp16 / bf16", TypeError)
+    _require(q.dim() == 3, lambda: f"q must be [tokens, heads, head_dim], got {tuple(q.shape)}")
+    t, hq, d = q.shape
+    q, k, v = _heads_view(q, "q", t, dtype, dev), _heads_view(k, "k", t, dtype, dev), _heads_view(v, "v", t, dtype, dev)
+    _require(k.shape == v.shape and k.shape[2] == d, lambda: f"k and v must both be [{t}, kv_heads, {d}]")
+    _require(k.shape[1] > 0 and hq % k.shape[1] == 0, lambda: f"{hq} q heads are not a multiple of {k.shape[1]} kv heads")
+    _on_gpu("log_decay", log_decay, torch.float32, dev)
+    _require(log_decay.dim() == 1 and log_decay.shape[0] == hq, lambda: f"log_decay must be [{hq}]")
+    log_decay = log_decay.contiguous()
+    _on_gpu("state", state, torch.float32, dev)
+    _require(state.dim() == 4 and tuple(state.shape[1:]) == (hq, d, d),
+             lambda: f"state must be [slots, {hq}, {d}, {d}], got {tuple(state.shape)}")
+    _require(state.stride(3) == 1 and state.stride(2) == d and state.stride(1) == d * d
+             and (state.shape[0] <= 1 or state.stride(0) >= hq * d * d), "state slots must be contiguous")
+    if state_slots is not None:
+        _on_gpu("state_slots", state_slots, torch.int32, dev)
+        _require(state_slots.dim() == 1 and state_slots.shape[0] == batch, lambda: f"state_slots must be [{batch}]")
+        state_slots = state_slots.contiguous()
+    if reset is not None:
+        _on_gpu("reset", reset, None, dev)
+        _require(reset.dtype in (torch.bool, torch.uint8), lambda: f"reset: dtype {reset.dtype} not in bool / uint8", TypeError)
+        _require(reset.dim() == 1 and reset.shape[0] == batch, lambda: f"reset must be [{batch}]")
+        reset = reset.contiguous()
+    args = (log_decay.data_ptr(), state.data_ptr(), state.stride(0) if state.shape[0] > 1 else hq * d * d, state.shape[0],
+            None if state_slots is None else state_slots.data_ptr(), None if reset is None else reset.data_ptr())
+    return q, k, v, _ROT_DTYPES[dtype], args, (log_decay, state_slots, reset)
+
+
+def linear_attn_varlen(q, k, v, log_decay, state, cu_seqlens, max_seqlen, *, state_slots=None, reset=None, scale):
+    """Causal linear attention of packed prompts (or draft chunks), one decay
+    per head: ``S <- exp(log_decay[h]) S + k_t v_t^T``, ``o_t = scale q_t^T S``.
+
+    ``q`` ``[T, Hq, D]``, ``k``, ``v`` ``[T, Hkv, D]`` fp16 or bf16;
+    ``log_decay`` fp32 ``[Hq]``, <= 0; ``cu_seqlens`` int32 ``[B + 1]``.
+    ``state``: fp32 pool ``[slots, Hq, D, D]`` (key dims by value dims),
+    updated in place: sequence b continues from slot ``state_slots[b]`` (int32
+    ``[B]``, default b; distinct) and leaves its state there; a slot outside
+    the pool marks a padding row (zeros out, no state).  ``reset`` (bool
+    ``[B]``): True starts from an empty state.  Returns ``[T, Hq, D]`` of q's
+    dtype; rows behind the last sequence are zeros."""
+    _on_gpu("q", q)
+    _on_gpu("cu_seqlens", cu_seqlens, torch.int32, q.device)
+    _require(cu_seqlens.dim() == 1 and cu_seqlens.numel() >= 1, "cu_seqlens must be [B + 1]")
+    cu_seqlens, b, max_seqlen = cu_seqlens.contiguous(), cu_seqlens.numel() - 1, int(max_seqlen)
+    _require(max_seqlen >= 0, "max_seqlen must be >= 0")
+    q, k, v, code, args, keep = _linear_args(q, k, v, log_decay, state, state_slots, reset, b)
+    t, hq, d = q.shape
+    out = torch.empty((t, hq, d), dtype=q.dtype, device=q.device)
+    if b == 0:
+        return out.zero_()
+    lib = _lib.load()
+    ws_bytes = int(lib.s8kv_linear_attn_workspace_size(b, hq, d, max_seqlen))
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
+    rc = _launch(q.device, lib.s8kv_linear_attn_varlen, q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0),
+                 k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), t, hq, k.shape[1], d, code, *args,
+                 cu_seqlens.data_ptr(), b, max_seqlen, scale, out.data_ptr(), hq * d, d,
+                 None if ws is None else ws.data_ptr(), ws_bytes, _stream(q))
+    _lib.check(rc, "linear_attn_varlen")
+    return out
+
+
+def linear_attn_decode(q, k, v, log_decay, state, *, state_slots=None, reset=None, scale):
+    """``linear_attn_varlen`` for one token per sequence: ``q`` ``[B, Hq, D]``,
+    ``k``, ``v`` ``[B, Hkv, D]``; returns ``[B, Hq, D]``."""
+    _on_gpu("q", q)
+    b = q.shape[0] if q.dim() else 0
+    q, k, v, code, args, keep = _linear_args(q, k, v, log_decay, state, state_slots, reset, b)
+    hq, d = q.shape[1:]
+    out = torch.empty((b, hq, d), dtype=q.dtype, device=q.device)
+    if b == 0:
+        return out
+    rc = _launch(q.device, _lib.load().s8kv_linear_attn_decode, q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(),
+                 k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), b, hq, k.shape[1], d, code, *args,
+                 scale, out.data_ptr(), hq * d, d, _stream(q))
+    _lib.check(rc, "linear_attn_decode")
+    return out

@@ -1,0 +1,311 @@
+"""Linear attention with a decay per head against the recurrence in 64 bits:
+lengths around the chunk edges, ragged batches, shared key heads, types,
+strides, slots, fresh and padding rows, extreme decays and values."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import layer_oracle as L
+from superl8_serve_amd import ops
+from tests.kvgpu import DEV, t, to_np
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = {"fp16": torch.float16, "bf16": torch.bfloat16}
+
+# What a result may be off, relative to the sum of its terms' absolute values
+# (q.k over D dims, tokens and the state's D rows): fp32 sums of at most D + 64
+# + D terms and 64 more for the state, 2^-24 each: 448 * 2^-24 < 2^-15.  Where
+# a matrix product takes fp32 values as two 16-bit halves, an fp16 pair is
+# within 2^-21, a bf16 pair within 2^-16 at worst; three such factors (decayed
+# scores, decayed values, the state) on top: fp16 3 * 2^-21 < 2^-19, bf16
+# 3 * 2^-16.  Sums: 2^-15 + 2^-19 and 2^-15 + 3 * 2^-16 < 2^-14 * 1.5.
+TERMS = {"fp16": 2.0 ** -15 + 2.0 ** -19, "bf16": 2.0 ** -15 + 3 * 2.0 ** -16}
+
+
+def inputs(rng, n, h, d, dtype, size=1.0):
+    return torch.from_numpy((rng.standard_normal((n, h, d)) * size).astype(np.float32)).to(dtype)
+
+
+def slopes(hq):
+    return -np.exp2(-8 * np.arange(1, hq + 1) / hq).astype(np.float32)
+
+
+def check(what, got, want, room, dtype=None):
+    """|got - want| within the terms' room, and half a step of the output's type."""
+    got = got.astype(np.float64)
+    half = 0.0 if dtype is None else torch.finfo(dtype).eps / 2 * np.abs(want) + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+    over = np.abs(got - want) - (room + half)
+    assert np.isfinite(got).all(), f"{what}: {np.isnan(got).sum()} NaN"
+    assert (over <= 0).all(), f"{what}: {over.max():.3e} over at {np.unravel_index(over.argmax(), over.shape)}"
+
+
+def expect(q, k, v, g, s0, scale, name):
+    """(out, state, room of each) of one sequence."""
+    f = [x.float().numpy() for x in (q, k, v)]
+    out, s = L.linear_attention(*f, g, s0, scale)
+    aout, as_ = L.linear_attention(*(np.abs(x) for x in f), g, np.abs(s0), abs(scale))
+    return out, s, aout * TERMS[name] + 1e-30, as_ * TERMS[name] + 1e-30
+
+
+def run(rng, lens, hq, hkv, d, name, g=None, size=1.0, scale=None, slots=None, reset=None, extra_rows=0, views=False):
+    dtype = DTYPES[name]
+    total, b = sum(lens) + extra_rows, len(lens)
+    scale = d ** -0.5 if scale is None else scale
+    g = slopes(hq) if g is None else np.asarray(g, np.float32)
+    q, k, v = (inputs(rng, total, h, d, dtype, size) for h in (hq, hkv, hkv))
+    state = rng.standard_normal((b + 2, hq, d, d)).astype(np.float32) * size * size
+    slots = rng.permutation(b + 2)[:b].astype(np.int32) if slots is None else np.asarray(slots, np.int32)
+    dev = [x.to(DEV) for x in (q, k, v)]
+    if views:  # slices of one projection
+        dev = list(torch.cat(dev, 1).split((hq, hkv, hkv), 1))
+    pool = t(state)
+    cu = np.concatenate([[0], np.cumsum(lens)]).astype(np.int32)
+    out = ops.linear_attn_varlen(*dev, t(g), pool, t(cu), max(lens, default=0), state_slots=t(slots),
+                                 reset=None if reset is None else t(np.asarray(reset, bool)), scale=scale)
+    got, new = out.float().cpu().numpy(), to_np(pool)
+    assert out.dtype == dtype
+    left = set(range(b + 2))
+    for i in range(b):
+        at = slice(cu[i], cu[i + 1])
+        if not 0 <= slots[i] < b + 2:
+            assert not got[at].any()
+            continue
+        left.discard(int(slots[i]))
+        s0 = state[slots[i]] * (0 if reset is not None and reset[i] else 1)
+        wo, ws, ro, rs = expect(q[at], k[at], v[at], g, s0, scale, name)
+        check(f"out of sequence {i} ({lens[i]} tokens)", got[at], wo, ro, dtype)
+        check(f"state of sequence {i} ({lens[i]} tokens)", new[slots[i]], ws, rs)
+    assert not got[cu[-1]:].any()
+    for s in left:
+        assert np.array_equal(new[s], state[s])
+
+
+@pytest.mark.parametrize("name", list(DTYPES))
+@pytest.mark.parametrize("d", [32, 64, 128, 256])
+def test_lengths(d, name):
+    rng = np.random.default_rng(d)
+    run(rng, [1, 2, 0, 31, 32, 33, 63, 64, 65, 127, 128, 129, 190], 4, 4, d, name)
+
+
+@pytest.mark.parametrize("name", list(DTYPES))
+@pytest.mark.parametrize("hq,hkv,d", [(1, 1, 128), (6, 2, 64), (8, 1, 128), (5, 5, 32), (4, 2, 256)])
+def test_heads_views_and_tail(hq, hkv, d, name):
+    rng = np.random.default_rng(hq + d)
+    run(rng, [70, 5, 200], hq, hkv, d, name, extra_rows=9, views=True)
+
+
+@pytest.mark.parametrize("name", list(DTYPES))
+@pytest.mark.parametrize("d", [64, 128])
+def test_long_and_lone(d, name):
+    """One sequence on few heads: the tokens are split over workgroups."""
+    rng = np.random.default_rng(d + 7)
+    run(rng, [3001], 2, 1, d, name)
+    run(rng, [1500, 17, 2100], 2, 2, d, name)
+
+
+@pytest.mark.parametrize("name", list(DTYPES))
+def test_slots_and_resets(name):
+    rng = np.random.default_rng(12)
+    run(rng, [5, 66, 130, 0, 0, 9], 2, 2, 128, name, slots=[3, -1, 0, 7, 8, 6], reset=[True, True, False, True, True, True])
+    run(rng, [1, 300], 4, 2, 64, name, slots=[2, 99], reset=[False, False])
+
+
+@pytest.mark.parametrize("name", list(DTYPES))
+@pytest.mark.parametrize("d", [64, 128])
+def test_extreme_decays(d, name):
+    rng = np.random.default_rng(d)
+    run(rng, [150, 64], 8, 8, d, name, g=[0.0, -1e-7, -1e-3, -1.0, -20.0, -90.0, -1e30, -np.inf])
+    run(rng, [2500], 2, 2, d, name, g=[0.0, -1e-4])
+
+
+@pytest.mark.parametrize("size", [1e-3, 60.0, 3000.0])
+def test_sizes_of_values(size):
+    """Products far outside fp16 in between; the scale brings them back."""
+    rng = np.random.default_rng(5)
+    run(rng, [200, 33], 2, 2, 128, "fp16", size=size, scale=0.005 / size ** 2)
+    run(rng, [200, 33], 2, 2, 128, "bf16", size=size, scale=0.005 / size ** 2)
+
+
+def test_unset_max_seqlen_is_only_a_hint():
+    rng = np.random.default_rng(3)
+    q, k, v = (inputs(rng, 400, 2, 64, torch.float16).to(DEV) for _ in range(3))
+    g, cu = t(slopes(2)), t(np.array([0, 390, 400], np.int32))
+    state = torch.zeros(2, 2, 64, 64, device=DEV)
+    want = ops.linear_attn_varlen(q, k, v, g, state.clone(), cu, 390, scale=0.1)
+    for hint in (0, 1, 100, 5000, 100000):
+        got = ops.linear_attn_varlen(q, k, v, g, state.clone(), cu, hint, scale=0.1)
+        assert (got.float() - want.float()).abs().max() <= 2e-3 * want.float().abs().max()
+
+
+@pytest.mark.parametrize("name", list(DTYPES))
+@pytest.mark.parametrize("what", ["v", "k", "q", "state"])
+def test_non_finite_values_reach_later_tokens_alone(what, name):
+    """A NaN or infinity at token 70 leaves the rows before it (of its chunk
+    too) and the other heads bit for bit as they are."""
+    rng = np.random.default_rng(17)
+    q, k, v = (inputs(rng, 200, 2, 128, DTYPES[name]).to(DEV) for _ in range(3))
+    g, cu = t(slopes(2)), t(np.array([0, 200], np.int32))
+    s0 = torch.randn(1, 2, 128, 128, device=DEV)
+    clean = ops.linear_attn_varlen(q, k, v, g, s0.clone(), cu, 200, scale=0.1).float().cpu()
+    for bad in (float("nan"), float("inf")):
+        x = {"q": q, "k": k, "v": v}
+        state = s0.clone()
+        if what == "state":
+            state[0, 1, 5, 9] = bad
+        else:
+            x[what] = x[what].clone()
+            x[what][70, 1, 9] = bad
+        got = ops.linear_attn_varlen(x["q"], x["k"], x["v"], g, state, cu, 200, scale=0.1).float().cpu()
+        assert (got[:, 0] - clean[:, 0]).abs().max() <= 2 ** -7 * clean[:, 0].abs().max()
+        assert torch.isfinite(got[:, 0]).all()
+        if what == "state":
+            assert torch.isfinite(got[:, 1, :9]).all() and torch.isfinite(got[:, 1, 10:]).all()
+            assert not torch.isfinite(got[:10, 1, 9]).any()
+            continue
+        assert torch.isfinite(got[:70]).all()
+        assert (got[:70] - clean[:70]).abs().max() <= 2 ** -7 * clean[:70].abs().max()
+        hit = got[70, 1, 9:10] if what == "v" else got[70, 1]
+        assert not torch.isfinite(hit).any()
+        if what == "q":
+            assert torch.isfinite(got[71:]).all() and torch.isfinite(state).all()
+        elif what == "v":
+            assert not torch.isfinite(got[71:80, 1, 9]).any()
+            assert torch.isfinite(got[70:, 1, :9]).all() and torch.isfinite(got[70:, 1, 10:]).all()
+
+
+@pytest.mark.parametrize("name", list(DTYPES))
+@pytest.mark.parametrize("b,hq,hkv,d", [(1, 1, 1, 32), (3, 8, 2, 64), (1, 32, 32, 128), (40, 6, 6, 128), (5, 4, 1, 256)])
+def test_decode(b, hq, hkv, d, name):
+    rng = np.random.default_rng(b + d)
+    dtype, scale = DTYPES[name], d ** -0.5
+    g = slopes(hq)
+    state = rng.standard_normal((b + 2, hq, d, d)).astype(np.float32)
+    slots = rng.permutation(b + 2)[:b].astype(np.int32)
+    reset = np.zeros(b, bool)
+    if b > 2:
+        slots[1], reset[2] = -1, True
+    pool = t(state)
+    for step in range(3):
+        q, k, v = (inputs(rng, b, h, d, dtype) for h in (hq, hkv, hkv))
+        dev = torch.cat([x.to(DEV) for x in (q, k, v)], 1).split((hq, hkv, hkv), 1)
+        out = ops.linear_attn_decode(*dev, t(g), pool, state_slots=t(slots), reset=t(reset), scale=scale)
+        got, new = out.float().cpu().numpy(), to_np(pool)
+        for i in range(b):
+            if slots[i] < 0:
+                assert not got[i].any()
+                continue
+            s0 = state[slots[i]] * (0 if reset[i] else 1)
+            wo, ws, ro, rs = expect(q[i:i + 1], k[i:i + 1], v[i:i + 1], g, s0, scale, name)
+            check(f"step {step} row {i}", got[i:i + 1], wo, ro, dtype)
+            check(f"step {step} state {i}", new[slots[i]], ws, rs)
+        for s in set(range(b + 2)) - set(slots.tolist()):
+            assert np.array_equal(new[s], state[s])
+        state = new
+
+
+def test_decode_drift():
+    """4,000 steps of a slow decay with nothing coming in: the decay's rounding
+    does not add up (one fp32 factor alone would be 4000 * 2^-25 off)."""
+    d, steps, g = 32, 4000, np.array([-1e-4], np.float32)
+    state = torch.ones(1, 1, d, d, device=DEV)
+    zero = torch.zeros(1, 1, d, dtype=torch.float16, device=DEV)
+    for _ in range(steps):
+        ops.linear_attn_decode(zero, zero, zero, t(g) if _ == 0 else dg, state, scale=1.0)
+        if _ == 0:
+            dg = t(g)
+    want = np.exp(np.float64(g[0]) * steps)
+    # each step rounds once (random sign): 6 sigma of 4000 roundings of 2^-25 uniform, and the pair's 2^-48
+    assert abs(float(state.double().mean()) / want - 1) <= 6 * np.sqrt(steps) * 2.0 ** -25
+    assert float((state.double() / want - 1).abs().max()) <= 6 * np.sqrt(steps) * 2.0 ** -25
+
+
+def test_prompt_in_pieces_equals_whole():
+    """A prompt, its chunks, and its tokens one by one leave the same state."""
+    rng = np.random.default_rng(23)
+    n, hq, d = 150, 3, 64
+    q, k, v = (inputs(rng, n, hq, d, torch.float16).to(DEV) for _ in range(3))
+    g = t(slopes(hq))
+    states = [torch.zeros(1, hq, d, d, device=DEV) for _ in range(3)]
+    cu = lambda m: t(np.array([0, m], np.int32))  # noqa: E731
+    whole = ops.linear_attn_varlen(q, k, v, g, states[0], cu(n), n, scale=0.125)
+    parts = [ops.linear_attn_varlen(q[a:b], k[a:b], v[a:b], g, states[1], cu(b - a), b - a, scale=0.125)
+             for a, b in ((0, 40), (40, 104), (104, 150))]
+    steps = [ops.linear_attn_decode(q[i:i + 1], k[i:i + 1], v[i:i + 1], g, states[2], scale=0.125) for i in range(n)]
+    room = 2 * TERMS["fp16"]
+    aout, astate = L.linear_attention(*(np.abs(x.float().cpu().numpy()) for x in (q, k, v)), to_np(g),
+                                      np.zeros((hq, d, d)), 0.125)
+    for other, state in ((torch.cat(parts), states[1]), (torch.cat(steps), states[2])):
+        diff = (other.double() - whole.double()).abs().cpu().numpy()
+        assert (diff <= room * aout + 2.0 ** -10 * np.abs(whole.double().cpu().numpy()) + 1e-7).all()
+        assert (np.abs(to_np(state).astype(np.float64) - to_np(states[0])) <= room * astate[None]).all()
+
+
+def test_captured_replays_and_two_streams():
+    """Two captured graphs, each with its own workspace, replayed in turn and
+    with eager calls between; then two streams at once."""
+    rng = np.random.default_rng(41)
+    g, cu = t(slopes(2)), t(np.array([0, 700, 2000], np.int32))
+    sets = []
+    for _ in range(2):
+        q, k, v = (inputs(rng, 2000, 2, 64, torch.float16).to(DEV) for _ in range(3))
+        state = torch.zeros(2, 2, 64, 64, device=DEV)
+        ops.linear_attn_varlen(q, k, v, g, state.clone(), cu, 1300, scale=0.1)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = ops.linear_attn_varlen(q, k, v, g, state, cu, 1300, scale=0.1)
+            step = ops.linear_attn_decode(q[:2], k[:2], v[:2], g, state, scale=0.1)
+        sets.append((q, k, v, state, graph, out, step))
+    for i in range(3):
+        for q, k, v, state, graph, out, step in sets:
+            q.copy_(inputs(rng, 2000, 2, 64, torch.float16))
+            eager = state.clone()
+            want = ops.linear_attn_varlen(q, k, v, g, eager, cu, 1300, scale=0.1)
+            want_step = ops.linear_attn_decode(q[:2], k[:2], v[:2], g, eager, scale=0.1)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want) and torch.equal(step, want_step) and torch.equal(state, eager), f"replay {i}"
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    want = [ops.linear_attn_varlen(*s[:3], g, s[3].clone(), cu, 1300, scale=0.1) for s in sets]
+    states = [s[3].clone() for s in sets]
+    torch.cuda.synchronize()
+    got = []
+    for stream, s, state in zip(streams, sets, states):
+        with torch.cuda.stream(stream):
+            got.append(ops.linear_attn_varlen(*s[:3], g, state, cu, 1300, scale=0.1))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_refusals():
+    n, hq, hkv, d = 6, 4, 2, 64
+    q, k, v = (torch.zeros(n, h, d, dtype=torch.float16, device=DEV) for h in (hq, hkv, hkv))
+    g, state = torch.zeros(hq, device=DEV), torch.zeros(3, hq, d, d, device=DEV)
+    cu = torch.tensor([0, 2, 6], dtype=torch.int32, device=DEV)
+    ok = dict(q=q, k=k, v=v, log_decay=g, state=state, cu_seqlens=cu, max_seqlen=4, scale=1.0)
+    for exc, change in [
+        (RuntimeError, dict(q=q.cpu())), (TypeError, dict(q=q.float())), (TypeError, dict(k=k.bfloat16())),
+        (ValueError, dict(k=k[:5])), (ValueError, dict(v=v[:, :1])), (ValueError, dict(k=k[:, :0], v=v[:, :0])),
+        (ValueError, dict(q=q[:, :3], log_decay=g[:3], state=state[:, :3])),
+        (ValueError, dict(log_decay=g[:2])), (TypeError, dict(log_decay=g.double())),
+        (TypeError, dict(state=state.half())), (ValueError, dict(state=state.transpose(2, 3))),
+        (ValueError, dict(state=state[:, :, :32])), (ValueError, dict(state=state[:1].expand(3, hq, d, d))),
+        (TypeError, dict(cu_seqlens=cu.long())), (ValueError, dict(cu_seqlens=cu[:0])), (ValueError, dict(max_seqlen=-1)),
+        (ValueError, dict(state_slots=cu)), (TypeError, dict(state_slots=cu[:2].long())),
+        (TypeError, dict(reset=cu[:2])), (ValueError, dict(reset=torch.zeros(3, dtype=torch.bool, device=DEV))),
+        (RuntimeError, dict(q=torch.zeros(n, 2, 96, dtype=torch.float16, device=DEV),
+                            k=torch.zeros(n, 2, 96, dtype=torch.float16, device=DEV),
+                            v=torch.zeros(n, 2, 96, dtype=torch.float16, device=DEV), log_decay=g[:2],
+                            state=torch.zeros(3, 2, 96, 96, device=DEV))),
+    ]:
+        with pytest.raises(exc):
+            ops.linear_attn_varlen(**{**ok, **change})
+    empty = ops.linear_attn_varlen(**{**ok, "cu_seqlens": cu[:1]})
+    assert empty.shape == q.shape and not empty.any()
+    with pytest.raises(ValueError):
+        ops.linear_attn_decode(q, k, v, g, state, state_slots=cu, scale=1.0)
+    assert ops.linear_attn_decode(q[:0], k[:0], v[:0], g, state, scale=1.0).shape == (0, hq, d)
