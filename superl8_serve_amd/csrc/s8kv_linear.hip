@@ -17,8 +17,7 @@ struct Args {
   int64_t q_t, q_h, k_t, k_h, v_t, v_h;
   void* out;
   int64_t o_t, o_h;
-  int64_t tokens;
-  int batch, heads, group;  // query heads, and of them those that share a key head
+  int tokens, batch, heads, group;  // query heads, and of them those that share a key head
   const float* log_decay;   // [heads]
   float* state;
   int64_t state_slot, num_slots;  // elements between slots
@@ -42,15 +41,18 @@ __device__ __forceinline__ void store1(void* p, int64_t i, float x) {
   else static_cast<__bf16*>(p)[i] = (__bf16)x;
 }
 
-// Tokens [first, last) of sequence b, clamped to the tensors.
-__device__ __forceinline__ void extent(const Args& a, int b, int64_t& first, int64_t& last) {
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+// Tokens [first, last) of sequence b, clamped to the tensors (cu_seqlens holds 32-bit counts).
+__device__ __forceinline__ void extent(const Args& a, int b, int& first, int& last) {
   first = b;
   last = b + 1;
   if (a.cu) {
-    first = min(max((int64_t)a.cu[b], (int64_t)0), a.tokens);
-    last = min(max((int64_t)a.cu[b + 1], first), a.tokens);
+    first = min(max(uniform(a.cu[b]), 0), a.tokens);
+    last = min(max(uniform(a.cu[b + 1]), first), a.tokens);
   }
 }
+// The first row behind the last sequence.
+__device__ __forceinline__ int behind(const Args& a) { return min(max(uniform(a.cu[a.batch]), 0), a.tokens); }
 
 // exp(x) as an fp32 pair hi + lo: a decay is applied thousands of times in a
 // row, and the rounding of a single fp32 factor would add up instead of
@@ -79,11 +81,11 @@ __global__ __launch_bounds__(256) void recurrent_kernel(Args a) {
   const int tid = threadIdx.x, tx = tid % TX, rg = tid / TX;
   const int col = tile * CT + 4 * tx;
 
-  int64_t first, last;
+  int first, last;
   extent(a, b, first, last);
-  const int slot = a.slots ? a.slots[b] : b;
+  const int slot = uniform(a.slots ? a.slots[b] : b);
   const bool live = slot >= 0 && slot < a.num_slots;
-  const bool fresh = live && a.reset && a.reset[b];
+  const bool fresh = live && a.reset && uniform(a.reset[b]);
   if (!live) {
     for (int64_t t = first; t < last; ++t)
       for (int c = tid; c < CT; c += 256) store1<DT>(a.out, t * a.o_t + h * a.o_h + tile * CT + c, 0.0f);
@@ -132,8 +134,7 @@ __global__ __launch_bounds__(256) void recurrent_kernel(Args a) {
     for (int i = 0; i < RPT; ++i) *reinterpret_cast<float4_t*>(st + (int64_t)(rg + RG * i) * D) = s[i];
   }
   if (a.cu) {  // rows behind the last sequence: zeros, shared out over the sequences' workgroups
-    const int64_t end = min(max((int64_t)a.cu[a.batch], (int64_t)0), a.tokens);
-    for (int64_t t = end + b; t < a.tokens; t += a.batch)
+    for (int64_t t = (int64_t)behind(a) + b; t < a.tokens; t += a.batch)
       for (int c = tid; c < CT; c += 256) store1<DT>(a.out, t * a.o_t + h * a.o_h + tile * CT + c, 0.0f);
   }
 }
@@ -160,17 +161,17 @@ static int launch(const Args& a, int head_dim, const char* what, hipStream_t str
 // ---------------------------------------------------------------------------
 // The chunked form, on the matrix cores
 // ---------------------------------------------------------------------------
-// Tokens i, j of a chunk of n (row i' = C - n + i of C: short chunks are
+// Tokens i, j of a chunk of n <= C (row i' = C - n + i: short chunks are
 // padded in front, so that every power of lambda below is the same in all):
 //   o_i = scale (sum_{j <= i} lambda^{i-j} (q_i . k_j) v_j + lambda^{i+1} q_i^T S),
 //   S <- lambda^n S + sum_j lambda^{n-1-j} k_j v_j^T.
 // A workgroup walks a sequence's (or a segment's) chunks for one head, its
 // D / 32 waves side by side over the value dims: a wave keeps its 32 columns
-// of S in fp32 accumulators, where they are the first operand of q^T S as
-// they stand (the accumulators' key dims come in groups of four, and q is
-// read in the same order).  The chunk's q, k, v go through LDS once; the next
+// of S in fp32 accumulators, where they are the first operand of S^T q^T as
+// they stand (the accumulators' key dims come in groups of four, and LDS holds
+// q's dims in that order).  The chunk's q, k, v go through LDS once; the next
 // chunk's loads are in flight meanwhile.  The C x C scores are made by up to
-// three waves, one 32 x 32 tile on or below the diagonal each, and shared
+// three waves, one 32 x 32 tile on or below the diagonal each, and exchanged
 // through LDS.  C is 64; 32 at head_dim 256, whose columns of S take 128
 // registers a lane.
 //
@@ -179,18 +180,19 @@ static int launch(const Args& a, int head_dim, const char* what, hipStream_t str
 // within 2^-22, bf16 within 2^-18 of the value), so that the state keeps fp32
 // grade and the output's only visible rounding is its last one; q, k and v
 // themselves are exact.  fp16 halves only reach from 2^-24 to 65504: scores,
-// state and values are scaled by powers of two that bring a bound of their
-// size to 2^15 (the scores: from the chunk's largest |q| and |k|; S: its
-// largest value; v and with it S as it is kept: the largest |v|, changed only
-// when a chunk's leaves [2^4, 2^15]).
+// state and values are scaled by powers of two that bring their largest value
+// below 2^15 (the scores': of a row of a tile; S's: of a wave's columns; v's,
+// and with it the scale that S is kept at: of the chunk, changed only when a
+// chunk's leaves [2^4, 2^15]).
 //
 // A masked score is zero, but zero times an infinite or NaN v of a later
-// token is not: a chunk with a non-finite value is redone token by token.
-typedef float float16_t __attribute__((ext_vector_type(16)));
+// token is not: a chunk whose v is not finite is redone token by token.
 typedef float float2_t __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
+
+typedef float float16_t __attribute__((ext_vector_type(16)));
 
 template <int D>
 constexpr int kChunk = D == 256 ? 32 : 64;
@@ -217,10 +219,22 @@ __device__ __forceinline__ float second(uint32_t w) {
   if constexpr (DT == 0) return (float)__builtin_bit_cast(half2_t, w)[1];
   else return __builtin_bit_cast(float, w & 0xFFFF0000u);
 }
+// a fa, b fb as 16-bit pairs hi + lo.  fp16: each half is one v_fma_mix, the
+// lower one the exact remainder's rounding (hi is pinned so that the
+// remainder reads it as it was packed).
 template <int DT>
-__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
-  hi = pack2<DT>(a, b);
-  lo = pack2<DT>(a - first<DT>(hi), b - second<DT>(hi));
+__device__ __forceinline__ void split2(float a, float fa, float b, float fb, uint32_t& hi, uint32_t& lo) {
+  if constexpr (DT == 0) {
+    hi = __builtin_bit_cast(uint32_t, half2_t{(_Float16)__builtin_fmaf(a, fa, 0.0f), (_Float16)__builtin_fmaf(b, fb, 0.0f)});
+    asm("" : "+v"(hi));
+    const half2_t h = __builtin_bit_cast(half2_t, hi);
+    lo = __builtin_bit_cast(uint32_t, half2_t{(_Float16)__builtin_fmaf(a, fa, -(float)h[0]),
+                                              (_Float16)__builtin_fmaf(b, fb, -(float)h[1])});
+  } else {
+    const float x = a * fa, y = b * fb;
+    hi = pack2<1>(x, y);
+    lo = pack2<1>(x - first<1>(hi), y - second<1>(hi));
+  }
 }
 __device__ __forceinline__ uint32_t pk_max(uint32_t a, uint32_t b) {
   return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2_t, a), __builtin_bit_cast(u16x2_t, b)));
@@ -236,22 +250,19 @@ __device__ __forceinline__ uint32_t wave_pk_max(uint32_t m) {
   const auto b = __builtin_amdgcn_permlane32_swap(m, m, false, false);
   return pk_max((uint32_t)b[0], (uint32_t)b[1]);
 }
-// The magnitude that 16 bits stand for (sign cleared), the largest finite one for inf and NaN.
-template <int DT>
+// The magnitude that fp16 bits stand for (sign cleared), the largest finite one for inf and NaN.
 __device__ __forceinline__ float magnitude(uint32_t bits) {
-  if constexpr (DT == 0) return (float)__builtin_bit_cast(_Float16, (uint16_t)min(bits, 0x7BFFu));
-  else return __builtin_bit_cast(float, min(bits, 0x7F7Fu) << 16);
+  return (float)__builtin_bit_cast(_Float16, (uint16_t)min(bits, 0x7BFFu));
 }
-// e such that values up to `bound` times 2^-e are below 2^top.
-__device__ __forceinline__ int excess(float bound, int top) {
-  return min(100, max(-100, (int)((__builtin_bit_cast(uint32_t, bound) >> 23) & 0xFFu) - 126 - top));
+// e such that values up to `bound` times 2^-e are below 2^15, at least `least`.
+__device__ __forceinline__ int excess(float bound, int least) {
+  return min(100, max(least, (int)((__builtin_bit_cast(uint32_t, bound) >> 23) & 0xFFu) - 141));
 }
-__device__ __forceinline__ float times_pow2(float x, int e) { return __builtin_amdgcn_ldexpf(x, e); }
+__device__ __forceinline__ float pow2(int e) { return __builtin_bit_cast(float, (uint32_t)(e + 127) << 23); }  // |e| <= 100
 
 // Segments of a sequence of `len` tokens: seg_len tokens each, the last one takes the rest.
-__device__ __forceinline__ int segments(const Args& a, int64_t len) {
-  const int64_t n = (len + a.seg_len - 1) / a.seg_len;
-  return (int)min(max(n, (int64_t)1), (int64_t)a.num_seg);
+__device__ __forceinline__ int segments(const Args& a, int len) {
+  return min(max((int)(((unsigned)len + a.seg_len - 1) / (unsigned)a.seg_len), 1), a.num_seg);
 }
 
 // OUT: outputs (from the segments' start states, where a sequence has
@@ -262,8 +273,9 @@ __global__ __launch_bounds__(2 * D, 2) void chunk_kernel(Args a) {
   constexpr int NW = D / 32, NT = 64 * NW, KT = D / 32;
   constexpr int C = kChunk<D>, IT = C / 32, T = C / 16;  // its 32-token tiles and 16-token steps
   constexpr int QP = 2 * D + 16, KP = 2 * D + 32, PP = 2 * C + 16;  // row pitches that spread a read's rows over the banks
-  constexpr int KO = OUT ? C * QP : 0, VO = KO + C * KP, PO = VO + C * KP, MO = PO + (OUT ? 2 * C * PP : 0);
-  constexpr int LO = MO + (8 * NW + 15) / 16 * 16;  // lambda^0 .. lambda^C, then lambda^(C - 1) .. lambda^0
+  constexpr int KO = OUT ? C * QP : 0, VO = KO + C * KP, PO = VO + C * KP, EO = PO + (OUT ? 2 * C * PP : 0);
+  constexpr int MO = EO + (OUT ? 3 * 32 * 4 : 0);  // (EO: the score rows' exponents by tile; MO: the waves' largest |v|)
+  constexpr int LO = MO + (4 * NW + 15) / 16 * 16 + 128;  // 32 ones, lambda^0 .. lambda^C, then 2^-sv lambda^(C - 1) .. lambda^0
   constexpr int LR = LO + 4 * (C + 4);
   __shared__ __attribute__((aligned(16))) char lds[LR + 4 * C];
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -272,76 +284,94 @@ __global__ __launch_bounds__(2 * D, 2) void chunk_kernel(Args a) {
   const int h = blockIdx.x % a.heads;
   const int seg = blockIdx.x / a.heads % a.num_seg;
   const int b = blockIdx.x / a.heads / a.num_seg;
-  int64_t first_t, last_t;
+  int first_t, last_t;
   extent(a, b, first_t, last_t);
-  const int slot = a.slots ? a.slots[b] : b;
+  const int slot = uniform(a.slots ? a.slots[b] : b);
   const bool live = slot >= 0 && slot < a.num_slots;
   const int nseg = segments(a, last_t - first_t);
-  char* const out = static_cast<char*>(a.out);
   if (OUT && seg == 0 && a.cu) {  // rows behind the last sequence: zeros, shared out over the sequences' workgroups
-    const int64_t end = min(max((int64_t)a.cu[a.batch], (int64_t)0), a.tokens);
-    for (int64_t t = end + b; t < a.tokens; t += a.batch)
+    for (int64_t t = (int64_t)behind(a) + b; t < a.tokens; t += a.batch)
       for (int c = tid; c < D; c += NT) store1<DT>(a.out, t * a.o_t + h * a.o_h + c, 0.0f);
   }
   if (seg >= nseg || (!OUT && seg == nseg - 1)) return;
-  int64_t pos = first_t + seg * (int64_t)a.seg_len;
-  const int64_t end = seg == nseg - 1 ? last_t : pos + a.seg_len;
+  int pos = first_t + seg * a.seg_len;
+  const int end = seg == nseg - 1 ? last_t : pos + a.seg_len;
   if (!live) {
     if constexpr (OUT)
       for (int64_t t = pos; t < end; ++t)
         for (int c = tid; c < D; c += NT) store1<DT>(a.out, t * a.o_t + h * a.o_h + c, 0.0f);
     return;
   }
-  const bool fresh = a.reset && a.reset[b];
+  const bool fresh = a.reset && uniform(a.reset[b]);
   if (pos >= end && !fresh) return;
   const int hk = h / a.group;
 
+  // ---- chunk loads through descriptors of the chunk's rows: the padding in front reads as zeros ----
+  const int lc = tid % (D / 8), lr = tid / (D / 8);
+  const uint32_t qs = 2 * (uint32_t)a.q_t, ks = 2 * (uint32_t)a.k_t, vs = 2 * (uint32_t)a.v_t;  // row strides in bytes
+  const uint32_t q_off = lr * qs + 16 * lc, k_off = lr * ks + 16 * lc, v_off = lr * vs + 16 * lc;
+  u32x4_t rq[T], rk[T], rv[T];
+  auto load = [&](int from, int len) {
+    const rsrc_t q = make_rsrc(static_cast<const uint16_t*>(a.q) + (int64_t)from * a.q_t + h * a.q_h, (len - 1) * qs + 2 * D);
+    const rsrc_t k = make_rsrc(static_cast<const uint16_t*>(a.k) + (int64_t)from * a.k_t + hk * a.k_h, (len - 1) * ks + 2 * D);
+    const rsrc_t v = make_rsrc(static_cast<const uint16_t*>(a.v) + (int64_t)from * a.v_t + hk * a.v_h, (len - 1) * vs + 2 * D);
+#pragma unroll
+    for (int i = 0; i < T; ++i) {
+      const uint32_t row = 16u * i - (uint32_t)(C - len);  // (a row before the first wraps to an offset past the end)
+      if constexpr (OUT) rq[i] = bload128(q, q_off + row * qs);
+      rk[i] = bload128(k, k_off + row * ks);
+      rv[i] = bload128(v, v_off + row * vs);
+    }
+  };
+  int single_until = pos;
+  int len = min(C, end - pos);
+  if (pos < end) load(pos, len);
+
+  // ---- powers of lambda ----
+  float* const pw = reinterpret_cast<float*>(lds + LO);
+  float* const left = reinterpret_cast<float*>(lds + LR);
+  const double gd = (double)a.log_decay[h];
+  if (tid < 32) pw[tid - 32] = 1.0f;  // (what masked scores meet)
+  for (int n = tid; n <= C; n += NT) {
+    const float x = (float)exp(n ? gd * n : 0.0);
+    pw[n] = x;
+    if (n < C) left[C - 1 - n] = x;
+  }
+  // lambda^C, of whose fp32 value's rounding 16 applications are made good at a time
+  const Factor lambda_c(gd * C);
+  const float drift = lambda_c.hi > 0.0f ? 16.0f * lambda_c.lo / lambda_c.hi : 0.0f;
+  int applied = 0;
+
   // ---- the state's columns 32 wv + l32: register r of tile mt is key dim 32 mt + 8 (r / 4) + 4 g + r % 4 ----
-  float* const pool = a.state + slot * a.state_slot + (int64_t)h * D * D;
-  float* const parts = a.parts + ((int64_t)b * a.heads + h) * a.num_seg * D * D;
+  const int64_t s_at = 4 * g * D + 32 * wv + l32;
+  float* const pool = a.state + slot * a.state_slot + (int64_t)h * D * D + s_at;
+  float* const parts = a.parts + ((int64_t)b * a.heads + h) * a.num_seg * D * D + s_at;
   float16_t S[KT];
-  {
-    const float* src = nseg > 1 ? parts + (int64_t)seg * D * D : pool;
-    const bool zero = !OUT || (nseg == 1 && fresh);
+  if (!OUT || (nseg == 1 && fresh)) {
 #pragma unroll
     for (int mt = 0; mt < KT; ++mt)
 #pragma unroll
-      for (int r = 0; r < 16; ++r)
-        S[mt][r] = zero ? 0.0f : src[(32 * mt + 8 * (r / 4) + 4 * g + r % 4) * D + 32 * wv + l32];
-  }
-
-  // ---- powers of lambda ----
-  const double gd = (double)a.log_decay[h];
-  const float g2 = fmaxf((float)(gd * 1.4426950408889634), -1e5f);  // (-inf: 0 x inf would be NaN)
-  float* const pw = reinterpret_cast<float*>(lds + LO);
-  for (int n = tid; n <= C; n += NT) {
-    const float x = exp2f(g2 * (float)n);
-    pw[n] = x;
-    if (n < C) reinterpret_cast<float*>(lds + LR)[C - 1 - n] = x;
-  }
-  int factor_len = C;
-  Factor lambda_n(gd * C);
-
-  // ---- chunk loads: 16 bytes of every 16th row a thread and tensor ----
-  const int lc = tid % (D / 8), lr = tid / (D / 8);
-  u32x4_t rq[T], rk[T], rv[T];
-  auto load = [&](int64_t from, int len) {
-    const int pad = C - len;
+      for (int r = 0; r < 16; ++r) S[mt][r] = 0.0f;
+  } else {
+    const float* src = nseg > 1 ? parts + (int64_t)seg * D * D : pool;
 #pragma unroll
-    for (int i = 0; i < T; ++i) {
-      const int row = lr + 16 * i;
-      rq[i] = rk[i] = rv[i] = u32x4_t{0, 0, 0, 0};
-      if (row >= pad) {
-        const int64_t t = from + row - pad;
-        if constexpr (OUT) rq[i] = *reinterpret_cast<const u32x4_t*>(static_cast<const uint16_t*>(a.q) + t * a.q_t + h * a.q_h + 8 * lc);
-        rk[i] = *reinterpret_cast<const u32x4_t*>(static_cast<const uint16_t*>(a.k) + t * a.k_t + hk * a.k_h + 8 * lc);
-        rv[i] = *reinterpret_cast<const u32x4_t*>(static_cast<const uint16_t*>(a.v) + t * a.v_t + hk * a.v_h + 8 * lc);
-      }
-    }
+    for (int mt = 0; mt < KT; ++mt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) S[mt][r] = src[(32 * mt + 8 * (r / 4) + r % 4) * D];
+  }
+
+  // operands: 8 values of a row (row l32 of the tile) and of a column (by
+  // transposed reads).  q rows hold their dims in the order of S's
+  // accumulators: of 16 dims 0-3, 8-11, 4-7, 12-15, so lane group g's eight are
+  // 4 g .. + 3 and 8 + 4 g .. + 3; k's are read to match.
+  auto q8 = [&](int it, int s) { return *reinterpret_cast<const u32x4_t*>(lds + (32 * it + l32) * QP + 32 * s + 16 * g); };
+  auto k8 = [&](int jt, int s) {
+    const char* p = lds + KO + (32 * jt + l32) * KP + 32 * s + 8 * g;
+    const u32x2_t x = *reinterpret_cast<const u32x2_t*>(p), y = *reinterpret_cast<const u32x2_t*>(p + 16);
+    return u32x4_t{x.x, x.y, y.x, y.y};
   };
-  // operands: 8 consecutive values of a row (rows l32 of the tile), and of a column by transposed reads
-  auto row8 = [&](int base, int pitch, int row, int col) {
-    return *reinterpret_cast<const u32x4_t*>(lds + base + row * pitch + 2 * col);
+  auto p8 = [&](int lo, int it, int t) {
+    return *reinterpret_cast<const u32x4_t*>(lds + PO + lo * C * PP + (32 * it + l32) * PP + 32 * t + 16 * g);
   };
   auto col8 = [&](int base, int t, int col) {  // rows 16 t + 8 g .. + 7 of column col + l32
     const char* p = lds + base + (16 * t + 8 * g + (li >> 2)) * KP + 2 * (col + 16 * ((lane >> 4) & 1) + 4 * (li & 3));
@@ -352,106 +382,110 @@ __global__ __launch_bounds__(2 * D, 2) void chunk_kernel(Args a) {
 
   int sv = 0;  // S is kept times 2^-sv, which brings v's largest value near 2^10 (fp16)
   bool first_chunk = true;
-  int64_t single_until = pos;
-  int len = (int)min((int64_t)C, end - pos);
-  if (pos < end) load(pos, len);
+  // (vmcnt 0: with the state's loads still counted as outstanding at the loop's head, the compiler waits for the
+  // loop's own loads where it overwrites registers that held the state's)
+  __builtin_amdgcn_s_waitcnt(0x0F70);
   while (pos < end) {
     // ---- stage ----
-    uint32_t mq = 0, mk = 0, mv = 0;
+    uint32_t mv = 0;
 #pragma unroll
     for (int i = 0; i < T; ++i) {
       const int row = lr + 16 * i;
+      if constexpr (OUT || DT == 0) {
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        if constexpr (OUT && DT == 0) {
-          mq = pk_max(mq, rq[i][w] & 0x7FFF7FFFu);
-          mk = pk_max(mk, rk[i][w] & 0x7FFF7FFFu);
-        }
-        if constexpr (OUT || DT == 0) mv = pk_max(mv, rv[i][w] & 0x7FFF7FFFu);
+        for (int w = 0; w < 4; ++w) mv = pk_max(mv, rv[i][w] & 0x7FFF7FFFu);
       }
-      if constexpr (OUT) *reinterpret_cast<u32x4_t*>(lds + row * QP + 16 * lc) = rq[i];
+      if constexpr (OUT) {
+        char* q = lds + row * QP + 32 * (lc / 2) + 8 * (lc % 2);
+        *reinterpret_cast<u32x2_t*>(q) = u32x2_t{rq[i][0], rq[i][1]};
+        *reinterpret_cast<u32x2_t*>(q + 16) = u32x2_t{rq[i][2], rq[i][3]};
+      }
       *reinterpret_cast<u32x4_t*>(lds + KO + row * KP + 16 * lc) = rk[i];
       *reinterpret_cast<u32x4_t*>(lds + VO + row * KP + 16 * lc) = rv[i];
     }
     if constexpr (OUT || DT == 0) {
-      const uint32_t a0 = wave_pk_max((pk_max(mq, mq >> 16) & 0xFFFFu) | pk_max(mk, mk >> 16) << 16);
-      const uint32_t a1 = wave_pk_max(pk_max(mv, mv >> 16));
-      if (lane == 0) *reinterpret_cast<u32x2_t*>(lds + MO + 8 * wv) = u32x2_t{a0, a1};
+      mv = wave_pk_max(pk_max(mv, mv >> 16));
+      if (lane == 0) *reinterpret_cast<uint32_t*>(lds + MO + 4 * wv) = mv;
     }
     __syncthreads();
-    float qkmax = 0.0f;
     if constexpr (OUT || DT == 0) {
-      uint32_t m0 = 0, m1 = 0;
+      uint32_t m = 0;
 #pragma unroll
-      for (int w = 0; w < NW; ++w) {
-        const u32x2_t m = *reinterpret_cast<const u32x2_t*>(lds + MO + 8 * w);
-        m0 = pk_max(m0, m.x);
-        m1 = pk_max(m1, m.y);
-      }
-      m0 = __builtin_amdgcn_readfirstlane((int)m0);
-      m1 = __builtin_amdgcn_readfirstlane((int)m1) & 0xFFFF;
-      constexpr uint32_t kInf = DT == 0 ? 0x7C00u : 0x7F80u;
-      if (OUT && len > 1 && ((m0 & 0xFFFFu) >= kInf || (m0 >> 16) >= kInf || m1 >= kInf)) {
+      for (int w = 0; w < NW; ++w) m = pk_max(m, *reinterpret_cast<const uint32_t*>(lds + MO + 4 * w));
+      m = (uint32_t)uniform((int)m) & 0xFFFFu;
+      if (OUT && len > 1 && m >= (DT == 0 ? 0x7C00u : 0x7F80u)) {
         single_until = pos + len;
         len = 1;
         __syncthreads();
         load(pos, 1);
+        __builtin_amdgcn_s_waitcnt(0x0F70);  // (as before the loop)
         continue;
       }
       if constexpr (DT == 0) {
-        qkmax = magnitude<0>(m0 & 0xFFFFu) * magnitude<0>(m0 >> 16);
-        const float vmax = magnitude<0>(m1);
-        if (first_chunk || (vmax > 0.0f && (times_pow2(vmax, -sv) < 16.0f || times_pow2(vmax, -sv) >= 32768.0f))) {
-          const int now = excess(vmax, 10);
+        const float vmax = magnitude(m), now_v = vmax * pow2(-sv);
+        if (first_chunk || (vmax > 0.0f && (now_v < 16.0f || now_v >= 32768.0f))) {
+          const int now = excess(vmax, -100) + 5;
 #pragma unroll
-          for (int mt = 0; mt < KT; ++mt)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) S[mt][r] = times_pow2(S[mt][r], sv - now);
+          for (int mt = 0; mt < KT; ++mt) S[mt] = S[mt] * pow2(sv) * pow2(-now);
           sv = now;
           first_chunk = false;
+          for (int n = tid; n < C; n += NT) left[n] = pw[C - 1 - n] * pow2(-sv);
+          __syncthreads();
         }
       }
     }
-    const int64_t next = pos + len;
-    const int next_len = next < single_until ? 1 : (int)min((int64_t)C, end - next);
+    const int next = pos + len;
+    const int next_len = next < single_until ? 1 : min(C, end - next);
     if (next < end) load(next, next_len);
-    if (len != factor_len) {
-      factor_len = len;
-      lambda_n = Factor(gd * len);
-    }
 
     u32x4_t vf[T];  // the wave's columns of v, 8 tokens a lane
     if constexpr (OUT) {
-      const int e = DT == 0 ? excess(qkmax * (float)D, 15) : 0;
       // ---- scores: rows j (key tokens), columns i; kept as P[i][j], hi and lo ----
-      auto tile = [&](int it, int jt) {
+      auto tile = [&](int it, int jt, int at) {
         float16_t acc = {};
 #pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks)
-          acc = mfma<DT>(row8(KO, KP, 32 * jt + l32, 16 * ks + 8 * g), row8(0, QP, 32 * it + l32, 16 * ks + 8 * g), acc);
+        for (int s0 = 0; s0 < D / 16; s0 += 4) {
+          constexpr int B = D / 16 < 4 ? D / 16 : 4;
+          u32x4_t kf[B], qf[B];
+#pragma unroll
+          for (int s = 0; s < B; ++s) {
+            kf[s] = k8(jt, s0 + s);
+            qf[s] = q8(it, s0 + s);
+          }
+#pragma unroll
+          for (int s = 0; s < B; ++s) acc = mfma<DT>(kf[s], qf[s], acc);
+        }
+        if (it == jt) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (l32 < 8 * (r / 4) + 4 * g + r % 4) acc[r] = 0.0f;
+        }
+        float down = 1.0f;
+        if constexpr (DT == 0) {
+          float m = 0.0f;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) m = fmaxf(m, fabsf(acc[r]));
+          const int e = excess(max_x32(m), -32);  // (products of fp16 values are 2^-48 or more; zeros must not drive e further)
+          down = pow2(-e);
+          if (g == 0) reinterpret_cast<int*>(lds + EO)[32 * at + l32] = e;
+        }
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          float p[4];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const int ago = 32 * (it - jt) + l32 - (8 * q + 4 * g + c);
-            p[c] = (DT == 0 ? times_pow2(acc[4 * q + c], -e) : acc[4 * q + c]) * pw[max(0, ago)];
-            if (it == jt && ago < 0) p[c] = 0.0f;
-          }
+          const float* d = pw + 32 * (it - jt) + l32 - 4 * g - 8 * q;
           uint32_t h0, h1, l0, l1;
-          split2<DT>(p[0], p[1], h0, l0);
-          split2<DT>(p[2], p[3], h1, l1);
-          char* at = lds + PO + (32 * it + l32) * PP + 2 * (32 * jt + 8 * q + 4 * g);
-          *reinterpret_cast<u32x2_t*>(at) = u32x2_t{h0, h1};
-          *reinterpret_cast<u32x2_t*>(at + C * PP) = u32x2_t{l0, l1};
+          split2<DT>(acc[4 * q], d[0] * down, acc[4 * q + 1], d[-1] * down, h0, l0);
+          split2<DT>(acc[4 * q + 2], d[-2] * down, acc[4 * q + 3], d[-3] * down, h1, l1);
+          char* to = lds + PO + (32 * it + l32) * PP + 2 * (32 * jt + 8 * q + 4 * g);
+          *reinterpret_cast<u32x2_t*>(to) = u32x2_t{h0, h1};
+          *reinterpret_cast<u32x2_t*>(to + C * PP) = u32x2_t{l0, l1};
         }
       };
-      if (wv == 0) tile(0, 0);
+      if (wv == 0) tile(0, 0, 0);
       if constexpr (IT == 2) {
-        if (wv == (NW < 4 ? 0 : 1)) tile(1, 1);
-        if (wv == (NW == 1 ? 0 : (NW == 2 ? 1 : 2))) tile(1, 0);
+        if (wv == (NW < 4 ? 0 : 1)) tile(1, 1, 1);
+        if (wv == (NW == 1 ? 0 : (NW == 2 ? 1 : 2))) tile(1, 0, 2);
       }
-      // ---- o^T = S^T q^T (rows: value dims, columns: tokens), then the tokens' decay ----
+      // ---- o^T = S^T q^T (rows: value dims, columns: tokens) ----
       float16_t O[IT] = {};
       int es = 0;
       if constexpr (DT == 0) {
@@ -468,63 +502,81 @@ __global__ __launch_bounds__(2 * D, 2) void chunk_kernel(Args a) {
           m = fmaxf(m, xor_partner<2>(m));
           m = fmaxf(m, xor_partner<4>(m));
           m = fmaxf(m, xor_partner<8>(m));
-          return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, max_x32(max_x16(m)))));
+          return __builtin_bit_cast(float, uniform(__builtin_bit_cast(int, max_x32(max_x16(m)))));
         };
         float m = largest(false);
         if (m == __builtin_inff()) m = largest(true);
-        es = excess(m, 15);
+        es = excess(m, -100);
       }
+      const float s_down = pow2(-es);
+      u32x4_t qf[2][IT], hi[2], lo[2];
+      auto halves = [&](int s) {
 #pragma unroll
-      for (int mt = 0; mt < KT; ++mt) {
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          u32x4_t hi, lo;
-#pragma unroll
-          for (int p = 0; p < 4; ++p) {
-            uint32_t x, y;
-            float s0 = S[mt][8 * s + 2 * p], s1 = S[mt][8 * s + 2 * p + 1];
-            if constexpr (DT == 0) {
-              s0 = times_pow2(s0, -es);
-              s1 = times_pow2(s1, -es);
-            }
-            split2<DT>(s0, s1, x, y);
-            hi[p] = x;
-            lo[p] = y;
-          }
-#pragma unroll
-          for (int it = 0; it < IT; ++it) {
-            const char* qp = lds + (32 * it + l32) * QP + 2 * (32 * mt + 16 * s + 4 * g);
-            const u32x2_t q0 = *reinterpret_cast<const u32x2_t*>(qp), q1 = *reinterpret_cast<const u32x2_t*>(qp + 16);
-            const u32x4_t qf = {q0.x, q0.y, q1.x, q1.y};
-            O[it] = mfma<DT>(hi, qf, O[it]);
-            O[it] = mfma<DT>(lo, qf, O[it]);
-          }
+        for (int p = 0; p < 4; ++p) {
+          uint32_t x, y;
+          split2<DT>(S[s / 2][8 * (s % 2) + 2 * p], s_down, S[s / 2][8 * (s % 2) + 2 * p + 1], s_down, x, y);
+          hi[s % 2][p] = x;
+          lo[s % 2][p] = y;
         }
-      }
+      };
+      // one step's reads and halves ahead, in the shadow of the step's MFMAs
 #pragma unroll
-      for (int it = 0; it < IT; ++it) O[it] *= times_pow2(pw[max(0, 32 * it + l32 + 1 - (C - len))], es + sv - e);
+      for (int it = 0; it < IT; ++it) qf[0][it] = q8(it, 0);
+      halves(0);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int s = 0; s < 2 * KT; ++s) {
+        if (s + 1 < 2 * KT) {
+#pragma unroll
+          for (int it = 0; it < IT; ++it) qf[(s + 1) % 2][it] = q8(it, s + 1);
+          halves(s + 1);
+        }
+#pragma unroll
+        for (int it = 0; it < IT; ++it) O[it] = mfma<DT>(hi[s % 2], qf[s % 2][it], O[it]);
+#pragma unroll
+        for (int it = 0; it < IT; ++it) O[it] = mfma<DT>(lo[s % 2], qf[s % 2][it], O[it]);
+        __builtin_amdgcn_sched_group_barrier(0x100, IT, 0);
+#pragma unroll
+        for (int n = 0; n < 2 * IT; ++n) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x002, IT == 2 ? 6 : 12, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
       __syncthreads();
-      // ---- + v^T P^T ----
+      // ---- times the tokens' decay, + v^T P^T ----
 #pragma unroll
-      for (int t = 0; t < T; ++t) {
-        vf[t] = col8(VO, t, 32 * wv);
-#pragma unroll
-        for (int it = 0; it < IT; ++it) {
-          if (16 * t >= 32 * (it + 1)) continue;
-          O[it] = mfma<DT>(vf[t], row8(PO, PP, 32 * it + l32, 16 * t + 8 * g), O[it]);
-          O[it] = mfma<DT>(vf[t], row8(PO + C * PP, PP, 32 * it + l32, 16 * t + 8 * g), O[it]);
-        }
-      }
-      const float up = times_pow2(a.scale, e);
+      for (int t = 0; t < T; ++t) vf[t] = col8(VO, t, 32 * wv);
 #pragma unroll
       for (int it = 0; it < IT; ++it) {
-        const int row = 32 * it + l32 - (C - len);
-        if (row >= 0) {
-          char* p = out + 2 * ((pos + row) * a.o_t + h * a.o_h + 32 * wv + 4 * g);
+        int e = 0, e1 = 0;  // the scores' exponents: of the row's first tile, and of its diagonal tile behind it
+        if constexpr (DT == 0) {
+          const int* ex = reinterpret_cast<const int*>(lds + EO) + l32;
+          e = ex[it == 0 ? 0 : 64];
+          if (it == 1) e1 = ex[32];
+        }
+        O[it] *= __builtin_amdgcn_ldexpf(pw[max(0, 32 * it + l32 + 1 - (C - len))], es + sv - e);
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
-            *reinterpret_cast<u32x2_t*>(p + 16 * q) = u32x2_t{pack2<DT>(O[it][4 * q] * up, O[it][4 * q + 1] * up),
-                                                              pack2<DT>(O[it][4 * q + 2] * up, O[it][4 * q + 3] * up)};
+        for (int t = 0; t < 2 * (it + 1); ++t) {
+          if (DT == 0 && t == 2) {
+            O[it] *= __builtin_amdgcn_ldexpf(1.0f, e - e1);
+            e = e1;
+          }
+          O[it] = mfma<DT>(vf[t], p8(0, it, t), O[it]);
+          O[it] = mfma<DT>(vf[t], p8(1, it, t), O[it]);
+        }
+        const float up = __builtin_amdgcn_ldexpf(a.scale, e);
+        const int row = 32 * it + l32 - (C - len);
+        // a lane pair (l, l + 32) holds value dims 8 q + 0 .. 3 and 4 .. 7 of a token; it trades two q's halves for 16-byte stores
+        uint16_t* o = static_cast<uint16_t*>(a.out) + (int64_t)(pos + row) * a.o_t + h * a.o_h + 32 * wv + 8 * g;
+#pragma unroll
+        for (int q = 0; q < 4; q += 2) {
+          const auto x = __builtin_amdgcn_permlane32_swap(pack2<DT>(O[it][4 * q] * up, O[it][4 * q + 1] * up),
+                                                          pack2<DT>(O[it][4 * q + 4] * up, O[it][4 * q + 5] * up), false, false);
+          const auto y = __builtin_amdgcn_permlane32_swap(pack2<DT>(O[it][4 * q + 2] * up, O[it][4 * q + 3] * up),
+                                                          pack2<DT>(O[it][4 * q + 6] * up, O[it][4 * q + 7] * up), false, false);
+          if (row >= 0)
+            *reinterpret_cast<u32x4_t*>(o + 8 * q) = u32x4_t{(uint32_t)x[0], (uint32_t)y[0], (uint32_t)x[1], (uint32_t)y[1]};
         }
       }
     } else {
@@ -532,28 +584,53 @@ __global__ __launch_bounds__(2 * D, 2) void chunk_kernel(Args a) {
       for (int t = 0; t < T; ++t) vf[t] = col8(VO, t, 32 * wv);
     }
     // ---- S <- lambda^n S + k^T (decayed v) ----
+    const float lambda_n = pw[len];
 #pragma unroll
-    for (int mt = 0; mt < KT; ++mt)
+    for (int mt = 0; mt < KT; ++mt) S[mt] *= lambda_n;
+    if (++applied == 16) {
+      applied = 0;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) S[mt][r] = lambda_n(S[mt][r]);
+      for (int mt = 0; mt < KT; ++mt)
 #pragma unroll
-    for (int t = 0; t < T; ++t) {
-      u32x4_t hi, lo;
-      const float4_t* w = reinterpret_cast<const float4_t*>(lds + LR + 4 * (16 * t + 8 * g));
+        for (int r = 0; r < 16; ++r) S[mt][r] = __builtin_fmaf(S[mt][r], drift, S[mt][r]);
+    }
+    constexpr int KB = KT < 4 ? KT : 4, KN = KT / KB;  // key tiles a batch of reads, batches a step
+    u32x4_t kf[2][KB], vh[2], vl[2];
+    auto decayed = [&](int t) {
+      const float4_t* w = reinterpret_cast<const float4_t*>(left + 16 * t + 8 * g);
+      const float4_t w0 = w[0], w1 = w[1];
 #pragma unroll
       for (int p = 0; p < 4; ++p) {
         uint32_t x, y;
-        split2<DT>(times_pow2(first<DT>(vf[t][p]), -sv) * w[p / 2][2 * p % 4],
-                   times_pow2(second<DT>(vf[t][p]), -sv) * w[p / 2][2 * p % 4 + 1], x, y);
-        hi[p] = x;
-        lo[p] = y;
+        split2<DT>(first<DT>(vf[t][p]), p < 2 ? w0[2 * p] : w1[2 * p - 4], second<DT>(vf[t][p]),
+                   p < 2 ? w0[2 * p + 1] : w1[2 * p - 3], x, y);
+        vh[t % 2][p] = x;
+        vl[t % 2][p] = y;
+      }
+    };
+#pragma unroll
+    for (int m = 0; m < KB; ++m) kf[0][m] = col8(KO, 0, 32 * m);
+    decayed(0);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int n = 0; n < T * KN; ++n) {
+      const int t = n / KN, m0 = n % KN * KB;
+      if (n + 1 < T * KN) {
+#pragma unroll
+        for (int m = 0; m < KB; ++m) kf[(n + 1) % 2][m] = col8(KO, (n + 1) / KN, 32 * ((n + 1) % KN * KB + m));
+        if ((n + 1) % KN == 0) decayed(t + 1);
       }
 #pragma unroll
-      for (int mt = 0; mt < KT; ++mt) {
-        const u32x4_t kf = col8(KO, t, 32 * mt);
-        S[mt] = mfma<DT>(kf, hi, S[mt]);
-        S[mt] = mfma<DT>(kf, lo, S[mt]);
+      for (int m = 0; m < KB; ++m) S[m0 + m] = mfma<DT>(kf[n % 2][m], vh[t % 2], S[m0 + m]);
+#pragma unroll
+      for (int m = 0; m < KB; ++m) S[m0 + m] = mfma<DT>(kf[n % 2][m], vl[t % 2], S[m0 + m]);
+      __builtin_amdgcn_sched_group_barrier(0x100, 2 * KB + 2, 0);
+#pragma unroll
+      for (int m = 0; m < 2 * KB; ++m) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
       }
+      __builtin_amdgcn_sched_barrier(0);
     }
     pos = next;
     len = next_len;
@@ -564,7 +641,8 @@ __global__ __launch_bounds__(2 * D, 2) void chunk_kernel(Args a) {
 #pragma unroll
   for (int mt = 0; mt < KT; ++mt)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) dst[(32 * mt + 8 * (r / 4) + 4 * g + r % 4) * D + 32 * wv + l32] = DT == 0 ? times_pow2(S[mt][r], sv) : S[mt][r];
+    for (int r = 0; r < 16; ++r)
+      dst[(32 * mt + 8 * (r / 4) + r % 4) * D] = DT == 0 ? __builtin_amdgcn_ldexpf(S[mt][r], sv) : S[mt][r];
 }
 
 // The segments' start states, in place over their contributions: part 0 takes
@@ -575,9 +653,9 @@ __global__ __launch_bounds__(256) void scan_kernel(Args a) {
   const int tile = blockIdx.x % TILES;
   const int h = blockIdx.x / TILES % a.heads;
   const int b = blockIdx.x / TILES / a.heads;
-  int64_t first_t, last_t;
+  int first_t, last_t;
   extent(a, b, first_t, last_t);
-  const int slot = a.slots ? a.slots[b] : b;
+  const int slot = uniform(a.slots ? a.slots[b] : b);
   const int nseg = segments(a, last_t - first_t);
   if (nseg == 1 || slot < 0 || slot >= a.num_slots) return;
   const int64_t at = 1024 * tile + 4 * threadIdx.x;
@@ -623,7 +701,10 @@ static int64_t parts_bytes(int batch, int heads, int head_dim, int num_seg) {
 
 template <int DT>
 static int launch_varlen(Args& a, int head_dim, const char* what, hipStream_t stream) {
-  auto rows = [](const void* p, int64_t t, int64_t h) { return (uintptr_t)p % 16 == 0 && t % 8 == 0 && h % 8 == 0; };
+  // (a chunk's rows have 32-bit offsets, one bit of them for the rows that are not there)
+  auto rows = [](const void* p, int64_t t, int64_t h) {
+    return (uintptr_t)p % 16 == 0 && t % 8 == 0 && h % 8 == 0 && t >= 0 && t < (1 << 24);
+  };
   if (!(rows(a.q, a.q_t, a.q_h) && rows(a.k, a.k_t, a.k_h) && rows(a.v, a.v_t, a.v_h) && rows(a.out, a.o_t, a.o_h)))
     return launch<DT>(a, head_dim, what, stream);
   switch (head_dim) {
@@ -642,6 +723,7 @@ static int fill(Args& a, const char* what, const void* q, int64_t q_t, int64_t q
                 int64_t o_t, int64_t o_h) {
   S8KV_REQUIRE(batch >= 0 && tokens >= 0, S8KV_ERR_INVALID, "%s: %d sequences, %lld tokens", what, batch,
                (long long)tokens);
+  S8KV_REQUIRE(tokens < (int64_t(1) << 31), S8KV_ERR_INVALID, "%s: %lld tokens are past 32 bits", what, (long long)tokens);
   S8KV_REQUIRE(num_q_heads > 0 && num_kv_heads > 0 && num_q_heads % num_kv_heads == 0, S8KV_ERR_INVALID,
                "%s: %d q heads are not a multiple of %d kv heads", what, num_q_heads, num_kv_heads);
   S8KV_REQUIRE(head_dim_ok(head_dim), S8KV_ERR_UNSUPPORTED, "%s: head_dim %d not in {32,64,128,256}", what, head_dim);
@@ -653,7 +735,7 @@ static int fill(Args& a, const char* what, const void* q, int64_t q_t, int64_t q
   S8KV_REQUIRE(num_slots == 0 || state, S8KV_ERR_INVALID, "%s: null state", what);
   S8KV_REQUIRE((uintptr_t)state % 16 == 0 && state_slot % 4 == 0, S8KV_ERR_INVALID,
                "%s: state slots must be 16-byte aligned", what);
-  a = Args{q, k, v, q_t, q_h, k_t, k_h, v_t, v_h, out, o_t, o_h, tokens, batch, num_q_heads,
+  a = Args{q, k, v, q_t, q_h, k_t, k_h, v_t, v_h, out, o_t, o_h, (int)tokens, batch, num_q_heads,
            num_q_heads / num_kv_heads, log_decay, state, state_slot, num_slots, slots, reset, nullptr, scale, 1, 1 << 30, nullptr};
   return S8KV_OK;
 }
