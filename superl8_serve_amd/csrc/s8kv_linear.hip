@@ -219,22 +219,14 @@ __device__ __forceinline__ float second(uint32_t w) {
   if constexpr (DT == 0) return (float)__builtin_bit_cast(half2_t, w)[1];
   else return __builtin_bit_cast(float, w & 0xFFFF0000u);
 }
-// a fa, b fb as 16-bit pairs hi + lo.  fp16: each half is one v_fma_mix, the
-// lower one the exact remainder's rounding (hi is pinned so that the
-// remainder reads it as it was packed).
+// a fa, b fb as 16-bit pairs hi + lo; lo takes the exact remainder.  (fp16:
+// v_fma_mixlo / mixhi would make each half in one instruction, but their
+// partial writes cost wait states; this way 26 % faster as a whole.)
 template <int DT>
 __device__ __forceinline__ void split2(float a, float fa, float b, float fb, uint32_t& hi, uint32_t& lo) {
-  if constexpr (DT == 0) {
-    hi = __builtin_bit_cast(uint32_t, half2_t{(_Float16)__builtin_fmaf(a, fa, 0.0f), (_Float16)__builtin_fmaf(b, fb, 0.0f)});
-    asm("" : "+v"(hi));
-    const half2_t h = __builtin_bit_cast(half2_t, hi);
-    lo = __builtin_bit_cast(uint32_t, half2_t{(_Float16)__builtin_fmaf(a, fa, -(float)h[0]),
-                                              (_Float16)__builtin_fmaf(b, fb, -(float)h[1])});
-  } else {
-    const float x = a * fa, y = b * fb;
-    hi = pack2<1>(x, y);
-    lo = pack2<1>(x - first<1>(hi), y - second<1>(hi));
-  }
+  hi = pack2<DT>(a * fa, b * fb);
+  asm("" : "+v"(hi));  // (the remainder reads hi as it was packed)
+  lo = pack2<DT>(__builtin_fmaf(a, fa, -first<DT>(hi)), __builtin_fmaf(b, fb, -second<DT>(hi)));
 }
 __device__ __forceinline__ uint32_t pk_max(uint32_t a, uint32_t b) {
   return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2_t, a), __builtin_bit_cast(u16x2_t, b)));
@@ -296,6 +288,11 @@ __global__ __launch_bounds__(2 * D, 2) void chunk_kernel(Args a) {
   if (seg >= nseg || (!OUT && seg == nseg - 1)) return;
   int pos = first_t + seg * a.seg_len;
   const int end = seg == nseg - 1 ? last_t : pos + a.seg_len;
+  if constexpr (!OUT) {
+    // tokens whose weight lambda^(tokens behind) is zero in fp32 (2^-160) add nothing to the segment's state
+    const float g2 = a.log_decay[h] * 1.4426950408889634f;
+    if (g2 < 0.0f) pos = max(pos, end - (int)fminf(160.0f / -g2 + 1.0f, 1e9f));
+  }
   if (!live) {
     if constexpr (OUT)
       for (int64_t t = pos; t < end; ++t)
@@ -439,6 +436,8 @@ __global__ __launch_bounds__(2 * D, 2) void chunk_kernel(Args a) {
     if (next < end) load(next, next_len);
 
     u32x4_t vf[T];  // the wave's columns of v, 8 tokens a lane
+    float16_t O[IT] = {};
+    int es = 0;
     if constexpr (OUT) {
       // ---- scores: rows j (key tokens), columns i; kept as P[i][j], hi and lo ----
       auto tile = [&](int it, int jt, int at) {
@@ -486,26 +485,34 @@ __global__ __launch_bounds__(2 * D, 2) void chunk_kernel(Args a) {
         if (wv == (NW == 1 ? 0 : (NW == 2 ? 1 : 2))) tile(1, 0, 2);
       }
       // ---- o^T = S^T q^T (rows: value dims, columns: tokens) ----
-      float16_t O[IT] = {};
-      int es = 0;
       if constexpr (DT == 0) {
+        // (magnitudes as integers: fmaxf would quiet every operand first)
         auto largest = [&](bool finite) {
-          float m = 0.0f;
+          uint32_t m = 0;
 #pragma unroll
           for (int mt = 0; mt < KT; ++mt)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-              const float x = fabsf(S[mt][r]);
-              m = fmaxf(m, finite && !(x < __builtin_inff()) ? 0.0f : x);
+              const float v = S[mt][r];  // (a copy: bit_cast of a vector's element reads element 0)
+              const uint32_t x = __builtin_bit_cast(uint32_t, v) & 0x7FFFFFFFu;
+              m = max(m, finite && x >= 0x7F800000u ? 0u : x);
             }
-          m = fmaxf(m, xor_partner<1>(m));
-          m = fmaxf(m, xor_partner<2>(m));
-          m = fmaxf(m, xor_partner<4>(m));
-          m = fmaxf(m, xor_partner<8>(m));
-          return __builtin_bit_cast(float, uniform(__builtin_bit_cast(int, max_x32(max_x16(m)))));
+          float f = __builtin_bit_cast(float, m);
+          auto wider = [&](float y) { f = __builtin_bit_cast(float, max(__builtin_bit_cast(uint32_t, f), __builtin_bit_cast(uint32_t, y))); };
+          wider(xor_partner<1>(f));
+          wider(xor_partner<2>(f));
+          wider(xor_partner<4>(f));
+          wider(xor_partner<8>(f));
+          LanePair p = lane_pair16(f);
+          f = p.a;
+          wider(p.b);
+          p = lane_pair32(f);
+          f = p.a;
+          wider(p.b);
+          return __builtin_bit_cast(float, uniform(__builtin_bit_cast(int, f)));
         };
         float m = largest(false);
-        if (m == __builtin_inff()) m = largest(true);
+        if (!(m < __builtin_inff())) m = largest(true);
         es = excess(m, -100);
       }
       const float s_down = pow2(-es);
@@ -543,46 +550,9 @@ __global__ __launch_bounds__(2 * D, 2) void chunk_kernel(Args a) {
         }
         __builtin_amdgcn_sched_barrier(0);
       }
-      __syncthreads();
-      // ---- times the tokens' decay, + v^T P^T ----
-#pragma unroll
-      for (int t = 0; t < T; ++t) vf[t] = col8(VO, t, 32 * wv);
-#pragma unroll
-      for (int it = 0; it < IT; ++it) {
-        int e = 0, e1 = 0;  // the scores' exponents: of the row's first tile, and of its diagonal tile behind it
-        if constexpr (DT == 0) {
-          const int* ex = reinterpret_cast<const int*>(lds + EO) + l32;
-          e = ex[it == 0 ? 0 : 64];
-          if (it == 1) e1 = ex[32];
-        }
-        O[it] *= __builtin_amdgcn_ldexpf(pw[max(0, 32 * it + l32 + 1 - (C - len))], es + sv - e);
-#pragma unroll
-        for (int t = 0; t < 2 * (it + 1); ++t) {
-          if (DT == 0 && t == 2) {
-            O[it] *= __builtin_amdgcn_ldexpf(1.0f, e - e1);
-            e = e1;
-          }
-          O[it] = mfma<DT>(vf[t], p8(0, it, t), O[it]);
-          O[it] = mfma<DT>(vf[t], p8(1, it, t), O[it]);
-        }
-        const float up = __builtin_amdgcn_ldexpf(a.scale, e);
-        const int row = 32 * it + l32 - (C - len);
-        // a lane pair (l, l + 32) holds value dims 8 q + 0 .. 3 and 4 .. 7 of a token; it trades two q's halves for 16-byte stores
-        uint16_t* o = static_cast<uint16_t*>(a.out) + (int64_t)(pos + row) * a.o_t + h * a.o_h + 32 * wv + 8 * g;
-#pragma unroll
-        for (int q = 0; q < 4; q += 2) {
-          const auto x = __builtin_amdgcn_permlane32_swap(pack2<DT>(O[it][4 * q] * up, O[it][4 * q + 1] * up),
-                                                          pack2<DT>(O[it][4 * q + 4] * up, O[it][4 * q + 5] * up), false, false);
-          const auto y = __builtin_amdgcn_permlane32_swap(pack2<DT>(O[it][4 * q + 2] * up, O[it][4 * q + 3] * up),
-                                                          pack2<DT>(O[it][4 * q + 6] * up, O[it][4 * q + 7] * up), false, false);
-          if (row >= 0)
-            *reinterpret_cast<u32x4_t*>(o + 8 * q) = u32x4_t{(uint32_t)x[0], (uint32_t)y[0], (uint32_t)x[1], (uint32_t)y[1]};
-        }
-      }
-    } else {
-#pragma unroll
-      for (int t = 0; t < T; ++t) vf[t] = col8(VO, t, 32 * wv);
     }
+#pragma unroll
+    for (int t = 0; t < T; ++t) vf[t] = col8(VO, t, 32 * wv);
     // ---- S <- lambda^n S + k^T (decayed v) ----
     const float lambda_n = pw[len];
 #pragma unroll
@@ -594,7 +564,7 @@ __global__ __launch_bounds__(2 * D, 2) void chunk_kernel(Args a) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) S[mt][r] = __builtin_fmaf(S[mt][r], drift, S[mt][r]);
     }
-    constexpr int KB = KT < 4 ? KT : 4, KN = KT / KB;  // key tiles a batch of reads, batches a step
+    constexpr int KB = KT < 2 ? KT : 2, KN = KT / KB;  // key tiles a batch of reads, batches a step
     u32x4_t kf[2][KB], vh[2], vl[2];
     auto decayed = [&](int t) {
       const float4_t* w = reinterpret_cast<const float4_t*>(left + 16 * t + 8 * g);
@@ -628,9 +598,45 @@ __global__ __launch_bounds__(2 * D, 2) void chunk_kernel(Args a) {
 #pragma unroll
       for (int m = 0; m < 2 * KB; ++m) {
         __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, 8 / KN > 2 ? 8 / KN : 2, 0);
       }
       __builtin_amdgcn_sched_barrier(0);
+    }
+    if constexpr (OUT) {
+      __syncthreads();
+      // ---- times the tokens' decay, + v^T P^T ----
+#pragma unroll
+      for (int it = 0; it < IT; ++it) {
+        int e = 0, e1 = 0;  // the scores' exponents: of the row's first tile, and of its diagonal tile behind it
+        if constexpr (DT == 0) {
+          const int* ex = reinterpret_cast<const int*>(lds + EO) + l32;
+          e = ex[it == 0 ? 0 : 64];
+          if (it == 1) e1 = ex[32];
+        }
+        O[it] *= __builtin_amdgcn_ldexpf(pw[max(0, 32 * it + l32 + 1 - (C - len))], es + sv - e);
+#pragma unroll
+        for (int t = 0; t < 2 * (it + 1); ++t) {
+          if (DT == 0 && t == 2) {
+            O[it] *= __builtin_amdgcn_ldexpf(1.0f, e - e1);
+            e = e1;
+          }
+          O[it] = mfma<DT>(vf[t], p8(0, it, t), O[it]);
+          O[it] = mfma<DT>(vf[t], p8(1, it, t), O[it]);
+        }
+        const float up = __builtin_amdgcn_ldexpf(a.scale, e);
+        const int row = 32 * it + l32 - (C - len);
+        // a lane pair (l, l + 32) holds value dims 8 q + 0 .. 3 and 4 .. 7 of a token; it trades two q's halves for 16-byte stores
+        uint16_t* o = static_cast<uint16_t*>(a.out) + (int64_t)(pos + row) * a.o_t + h * a.o_h + 32 * wv + 8 * g;
+#pragma unroll
+        for (int q = 0; q < 4; q += 2) {
+          const auto x = __builtin_amdgcn_permlane32_swap(pack2<DT>(O[it][4 * q] * up, O[it][4 * q + 1] * up),
+                                                          pack2<DT>(O[it][4 * q + 4] * up, O[it][4 * q + 5] * up), false, false);
+          const auto y = __builtin_amdgcn_permlane32_swap(pack2<DT>(O[it][4 * q + 2] * up, O[it][4 * q + 3] * up),
+                                                          pack2<DT>(O[it][4 * q + 6] * up, O[it][4 * q + 7] * up), false, false);
+          if (row >= 0)
+            *reinterpret_cast<u32x4_t*>(o + 8 * q) = u32x4_t{(uint32_t)x[0], (uint32_t)y[0], (uint32_t)x[1], (uint32_t)y[1]};
+        }
+      }
     }
     pos = next;
     len = next_len;
