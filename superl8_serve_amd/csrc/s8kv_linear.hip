@@ -265,8 +265,9 @@ __global__ __launch_bounds__(2 * D, 2) void chunk_kernel(Args a) {
   constexpr int NW = D / 32, NT = 64 * NW, KT = D / 32;
   constexpr int C = kChunk<D>, IT = C / 32, T = C / 16;  // its 32-token tiles and 16-token steps
   constexpr int QP = 2 * D + 16, KP = 2 * D + 32, PP = 2 * C + 16;  // row pitches that spread a read's rows over the banks
-  constexpr int KO = OUT ? C * QP : 0, VO = KO + C * KP, PO = VO + C * KP, EO = PO + (OUT ? 2 * C * PP : 0);
-  constexpr int MO = EO + (OUT ? 3 * 32 * 4 : 0);  // (EO: the score rows' exponents by tile; MO: the waves' largest |v|)
+  constexpr int PH = IT == 1 ? 64 * PP : C * PP;  // bytes of the scores' hi halves (and of lo; with one tile, room for a second)
+  constexpr int KO = OUT ? C * QP : 0, VO = KO + C * KP, PO = VO + C * KP, EO = PO + (OUT ? 2 * PH : 0);
+  constexpr int MO = EO + (OUT ? 4 * 32 * 4 : 0);  // (EO: the score rows' exponents by tile; MO: the waves' largest |v|)
   constexpr int LO = MO + (4 * NW + 15) / 16 * 16 + 128;  // 32 ones, lambda^0 .. lambda^C, then 2^-sv lambda^(C - 1) .. lambda^0
   constexpr int LR = LO + 4 * (C + 4);
   __shared__ __attribute__((aligned(16))) char lds[LR + 4 * C];
@@ -368,7 +369,7 @@ __global__ __launch_bounds__(2 * D, 2) void chunk_kernel(Args a) {
     return u32x4_t{x.x, x.y, y.x, y.y};
   };
   auto p8 = [&](int lo, int it, int t) {
-    return *reinterpret_cast<const u32x4_t*>(lds + PO + lo * C * PP + (32 * it + l32) * PP + 32 * t + 16 * g);
+    return *reinterpret_cast<const u32x4_t*>(lds + PO + lo * PH + (32 * it + l32) * PP + 32 * t + 16 * g);
   };
   auto col8 = [&](int base, int t, int col) {  // rows 16 t + 8 g .. + 7 of column col + l32
     const char* p = lds + base + (16 * t + 8 * g + (li >> 2)) * KP + 2 * (col + 16 * ((lane >> 4) & 1) + 4 * (li & 3));
@@ -379,9 +380,41 @@ __global__ __launch_bounds__(2 * D, 2) void chunk_kernel(Args a) {
 
   int sv = 0;  // S is kept times 2^-sv, which brings v's largest value near 2^10 (fp16)
   bool first_chunk = true;
+  // the largest finite |S| of the wave (magnitudes as integers: fmaxf would quiet every operand first)
+  auto largest = [&]() {
+    auto of = [&](bool finite) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int mt = 0; mt < KT; ++mt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const float v = S[mt][r];  // (a copy: bit_cast of a vector's element reads element 0)
+          const uint32_t x = __builtin_bit_cast(uint32_t, v) & 0x7FFFFFFFu;
+          m = max(m, finite && x >= 0x7F800000u ? 0u : x);
+        }
+      auto wider = [&](float y) { m = max(m, __builtin_bit_cast(uint32_t, y)); };
+      auto f = [&]() { return __builtin_bit_cast(float, m); };
+      wider(xor_partner<1>(f()));
+      wider(xor_partner<2>(f()));
+      wider(xor_partner<4>(f()));
+      wider(xor_partner<8>(f()));
+      const auto x = __builtin_amdgcn_permlane16_swap(m, m, false, false);
+      m = max((uint32_t)x[0], (uint32_t)x[1]);
+      const auto y = __builtin_amdgcn_permlane32_swap(m, m, false, false);
+      return (uint32_t)uniform((int)max((uint32_t)y[0], (uint32_t)y[1]));
+    };
+    uint32_t m = of(false);
+    if (m >= 0x7F800000u) m = of(true);
+    return __builtin_bit_cast(float, m);
+  };
+  // the wave's score tile: (0, 0), (1, 1) and (1, 0) by wave; waves without one make one that is not read
+  const int my_at = IT == 1 ? (wv == 0 ? 0 : 3) : (NW == 2 ? 2 * wv : (wv < 3 ? wv : 3));
+  const int my_it = IT == 1 ? (wv == 0 ? 0 : 1) : (my_at == 1 || my_at == 2), my_jt = IT == 1 ? 0 : (my_at == 1 || my_at == 3);
   // (vmcnt 0: with the state's loads still counted as outstanding at the loop's head, the compiler waits for the
   // loop's own loads where it overwrites registers that held the state's)
   __builtin_amdgcn_s_waitcnt(0x0F70);
+  float s_max = 0.0f;
+  if constexpr (OUT && DT == 0) s_max = largest();
   while (pos < end) {
     // ---- stage ----
     uint32_t mv = 0;
@@ -424,6 +457,7 @@ __global__ __launch_bounds__(2 * D, 2) void chunk_kernel(Args a) {
           const int now = excess(vmax, -100) + 5;
 #pragma unroll
           for (int mt = 0; mt < KT; ++mt) S[mt] = S[mt] * pow2(sv) * pow2(-now);
+          s_max = s_max * pow2(sv) * pow2(-now);
           sv = now;
           first_chunk = false;
           for (int n = tid; n < C; n += NT) left[n] = pw[C - 1 - n] * pow2(-sv);
@@ -436,85 +470,55 @@ __global__ __launch_bounds__(2 * D, 2) void chunk_kernel(Args a) {
     if (next < end) load(next, next_len);
 
     u32x4_t vf[T];  // the wave's columns of v, 8 tokens a lane
-    float16_t O[IT] = {};
-    int es = 0;
-    if constexpr (OUT) {
-      // ---- scores: rows j (key tokens), columns i; kept as P[i][j], hi and lo ----
-      auto tile = [&](int it, int jt, int at) {
-        float16_t acc = {};
+    float16_t O[IT] = {}, P = {};
+    const int es = DT == 0 ? excess(s_max, -100) : 0;
+    const float lambda_n = pw[len];
+    float down = 1.0f;
+    // A tile of the scores (rows j: key tokens, columns i), done in three
+    // parts: its MFMAs; the mask and the rows' exponents; P[i][j] of four
+    // times eight key tokens, hi and lo.
+    auto masked = [&](float16_t& acc, int diag, int at) {
+      const int lim = diag ? l32 : C;
 #pragma unroll
-        for (int s0 = 0; s0 < D / 16; s0 += 4) {
-          constexpr int B = D / 16 < 4 ? D / 16 : 4;
-          u32x4_t kf[B], qf[B];
-#pragma unroll
-          for (int s = 0; s < B; ++s) {
-            kf[s] = k8(jt, s0 + s);
-            qf[s] = q8(it, s0 + s);
-          }
-#pragma unroll
-          for (int s = 0; s < B; ++s) acc = mfma<DT>(kf[s], qf[s], acc);
-        }
-        if (it == jt) {
-#pragma unroll
-          for (int r = 0; r < 16; ++r)
-            if (l32 < 8 * (r / 4) + 4 * g + r % 4) acc[r] = 0.0f;
-        }
-        float down = 1.0f;
-        if constexpr (DT == 0) {
-          float m = 0.0f;
-#pragma unroll
-          for (int r = 0; r < 16; ++r) m = fmaxf(m, fabsf(acc[r]));
-          const int e = excess(max_x32(m), -32);  // (products of fp16 values are 2^-48 or more; zeros must not drive e further)
-          down = pow2(-e);
-          if (g == 0) reinterpret_cast<int*>(lds + EO)[32 * at + l32] = e;
-        }
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const float* d = pw + 32 * (it - jt) + l32 - 4 * g - 8 * q;
-          uint32_t h0, h1, l0, l1;
-          split2<DT>(acc[4 * q], d[0] * down, acc[4 * q + 1], d[-1] * down, h0, l0);
-          split2<DT>(acc[4 * q + 2], d[-2] * down, acc[4 * q + 3], d[-3] * down, h1, l1);
-          char* to = lds + PO + (32 * it + l32) * PP + 2 * (32 * jt + 8 * q + 4 * g);
-          *reinterpret_cast<u32x2_t*>(to) = u32x2_t{h0, h1};
-          *reinterpret_cast<u32x2_t*>(to + C * PP) = u32x2_t{l0, l1};
-        }
-      };
-      if (wv == 0) tile(0, 0, 0);
-      if constexpr (IT == 2) {
-        if (wv == (NW < 4 ? 0 : 1)) tile(1, 1, 1);
-        if (wv == (NW == 1 ? 0 : (NW == 2 ? 1 : 2))) tile(1, 0, 2);
-      }
-      // ---- o^T = S^T q^T (rows: value dims, columns: tokens) ----
+      for (int r = 0; r < 16; ++r)
+        if (lim < 8 * (r / 4) + 4 * g + r % 4) acc[r] = 0.0f;
       if constexpr (DT == 0) {
-        // (magnitudes as integers: fmaxf would quiet every operand first)
-        auto largest = [&](bool finite) {
-          uint32_t m = 0;
+        uint32_t m = 0;
 #pragma unroll
-          for (int mt = 0; mt < KT; ++mt)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-              const float v = S[mt][r];  // (a copy: bit_cast of a vector's element reads element 0)
-              const uint32_t x = __builtin_bit_cast(uint32_t, v) & 0x7FFFFFFFu;
-              m = max(m, finite && x >= 0x7F800000u ? 0u : x);
-            }
-          float f = __builtin_bit_cast(float, m);
-          auto wider = [&](float y) { f = __builtin_bit_cast(float, max(__builtin_bit_cast(uint32_t, f), __builtin_bit_cast(uint32_t, y))); };
-          wider(xor_partner<1>(f));
-          wider(xor_partner<2>(f));
-          wider(xor_partner<4>(f));
-          wider(xor_partner<8>(f));
-          LanePair p = lane_pair16(f);
-          f = p.a;
-          wider(p.b);
-          p = lane_pair32(f);
-          f = p.a;
-          wider(p.b);
-          return __builtin_bit_cast(float, uniform(__builtin_bit_cast(int, f)));
-        };
-        float m = largest(false);
-        if (!(m < __builtin_inff())) m = largest(true);
-        es = excess(m, -100);
+        for (int r = 0; r < 16; ++r) {
+          const float x = acc[r];
+          m = max(m, __builtin_bit_cast(uint32_t, x) & 0x7FFFFFFFu);
+        }
+        const auto x = __builtin_amdgcn_permlane32_swap(m, m, false, false);
+        // (products of fp16 values are 2^-48 or more; a row of zeros must not drive its exponent further)
+        const int e = excess(__builtin_bit_cast(float, max((uint32_t)x[0], (uint32_t)x[1])), -32);
+        down = pow2(-e);
+        reinterpret_cast<int*>(lds + EO)[32 * at + l32] = e;
       }
+    };
+    auto exchanged = [&](const float16_t& acc, int it, int jt, int q) {
+      const float* d = pw + 32 * (it - jt) + l32 - 4 * g - 8 * q;
+      uint32_t h0, h1, l0, l1;
+      split2<DT>(acc[4 * q], d[0] * down, acc[4 * q + 1], d[-1] * down, h0, l0);
+      split2<DT>(acc[4 * q + 2], d[-2] * down, acc[4 * q + 3], d[-3] * down, h1, l1);
+      char* to = lds + PO + (32 * it + l32) * PP + 2 * (32 * jt + 8 * q + 4 * g);
+      *reinterpret_cast<u32x2_t*>(to) = u32x2_t{h0, h1};
+      *reinterpret_cast<u32x2_t*>(to + PH) = u32x2_t{l0, l1};
+    };
+    if constexpr (OUT) {
+      if constexpr (NW < 3 && IT == 2) {  // the tiles that the waves have no turn for below
+        auto tile = [&](int it, int jt, int at) {
+          float16_t acc = {};
+#pragma unroll
+          for (int s = 0; s < D / 16; ++s) acc = mfma<DT>(k8(jt, s), q8(it, s), acc);
+          masked(acc, it == jt, at);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) exchanged(acc, it, jt, q);
+        };
+        if (wv == 0) tile(1, 1, 1);
+        if (NW == 1) tile(1, 0, 2);
+      }
+      // ---- o^T = S^T q^T (rows: value dims, columns: tokens), and the wave's score tile ----
       const float s_down = pow2(-es);
       u32x4_t qf[2][IT], hi[2], lo[2];
       auto halves = [&](int s) {
@@ -526,37 +530,40 @@ __global__ __launch_bounds__(2 * D, 2) void chunk_kernel(Args a) {
           lo[s % 2][p] = y;
         }
       };
-      // one step's reads and halves ahead, in the shadow of the step's MFMAs
+      // one step's reads and halves ahead, and S's decay behind, in the shadow of the step's MFMAs
 #pragma unroll
       for (int it = 0; it < IT; ++it) qf[0][it] = q8(it, 0);
       halves(0);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int s = 0; s < 2 * KT; ++s) {
+        const u32x4_t kp = k8(my_jt, s), qp = q8(my_it, s);
         if (s + 1 < 2 * KT) {
 #pragma unroll
           for (int it = 0; it < IT; ++it) qf[(s + 1) % 2][it] = q8(it, s + 1);
           halves(s + 1);
         }
+        if (s % 2) S[s / 2] *= lambda_n;
 #pragma unroll
         for (int it = 0; it < IT; ++it) O[it] = mfma<DT>(hi[s % 2], qf[s % 2][it], O[it]);
 #pragma unroll
         for (int it = 0; it < IT; ++it) O[it] = mfma<DT>(lo[s % 2], qf[s % 2][it], O[it]);
-        __builtin_amdgcn_sched_group_barrier(0x100, IT, 0);
+        P = mfma<DT>(kp, qp, P);
+        __builtin_amdgcn_sched_group_barrier(0x100, IT + 3, 0);
 #pragma unroll
-        for (int n = 0; n < 2 * IT; ++n) {
+        for (int n = 0; n < 2 * IT + 1; ++n) {
           __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-          __builtin_amdgcn_sched_group_barrier(0x002, IT == 2 ? 6 : 12, 0);
+          __builtin_amdgcn_sched_group_barrier(0x002, IT == 2 ? 8 : 12, 0);
         }
         __builtin_amdgcn_sched_barrier(0);
       }
+    } else {
+#pragma unroll
+      for (int mt = 0; mt < KT; ++mt) S[mt] *= lambda_n;
     }
 #pragma unroll
     for (int t = 0; t < T; ++t) vf[t] = col8(VO, t, 32 * wv);
-    // ---- S <- lambda^n S + k^T (decayed v) ----
-    const float lambda_n = pw[len];
-#pragma unroll
-    for (int mt = 0; mt < KT; ++mt) S[mt] *= lambda_n;
+    // ---- S <- lambda^n S (done) + k^T (decayed v), and the tile's exchange ----
     if (++applied == 16) {
       applied = 0;
 #pragma unroll
@@ -564,7 +571,7 @@ __global__ __launch_bounds__(2 * D, 2) void chunk_kernel(Args a) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) S[mt][r] = __builtin_fmaf(S[mt][r], drift, S[mt][r]);
     }
-    constexpr int KB = KT < 2 ? KT : 2, KN = KT / KB;  // key tiles a batch of reads, batches a step
+    constexpr int KB = KT < 2 ? KT : 2, KN = KT / KB, N = T * KN;  // key tiles a batch of reads, batches a step, batches
     u32x4_t kf[2][KB], vh[2], vl[2];
     auto decayed = [&](int t) {
       const float4_t* w = reinterpret_cast<const float4_t*>(left + 16 * t + 8 * g);
@@ -581,49 +588,62 @@ __global__ __launch_bounds__(2 * D, 2) void chunk_kernel(Args a) {
 #pragma unroll
     for (int m = 0; m < KB; ++m) kf[0][m] = col8(KO, 0, 32 * m);
     decayed(0);
+    if constexpr (OUT) masked(P, my_it == my_jt, my_at);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int n = 0; n < T * KN; ++n) {
+    for (int n = 0; n < N; ++n) {
       const int t = n / KN, m0 = n % KN * KB;
-      if (n + 1 < T * KN) {
+      if (n + 1 < N) {
 #pragma unroll
         for (int m = 0; m < KB; ++m) kf[(n + 1) % 2][m] = col8(KO, (n + 1) / KN, 32 * ((n + 1) % KN * KB + m));
         if ((n + 1) % KN == 0) decayed(t + 1);
+      }
+      if constexpr (OUT) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (q * N / 4 == n) exchanged(P, my_it, my_jt, q);
       }
 #pragma unroll
       for (int m = 0; m < KB; ++m) S[m0 + m] = mfma<DT>(kf[n % 2][m], vh[t % 2], S[m0 + m]);
 #pragma unroll
       for (int m = 0; m < KB; ++m) S[m0 + m] = mfma<DT>(kf[n % 2][m], vl[t % 2], S[m0 + m]);
-      __builtin_amdgcn_sched_group_barrier(0x100, 2 * KB + 2, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 2 * KB + 4, 0);
 #pragma unroll
       for (int m = 0; m < 2 * KB; ++m) {
         __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x002, 8 / KN > 2 ? 8 / KN : 2, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, 8, 0);
       }
       __builtin_amdgcn_sched_barrier(0);
     }
     if constexpr (OUT) {
       __syncthreads();
       // ---- times the tokens' decay, + v^T P^T ----
+      int e[IT], e1 = 0;  // the scores' exponents: of a row's first tile, and of its diagonal tile behind it
 #pragma unroll
       for (int it = 0; it < IT; ++it) {
-        int e = 0, e1 = 0;  // the scores' exponents: of the row's first tile, and of its diagonal tile behind it
+        e[it] = 0;
         if constexpr (DT == 0) {
           const int* ex = reinterpret_cast<const int*>(lds + EO) + l32;
-          e = ex[it == 0 ? 0 : 64];
+          e[it] = ex[it == 0 ? 0 : 64];
           if (it == 1) e1 = ex[32];
         }
-        O[it] *= __builtin_amdgcn_ldexpf(pw[max(0, 32 * it + l32 + 1 - (C - len))], es + sv - e);
+        O[it] *= __builtin_amdgcn_ldexpf(pw[max(0, 32 * it + l32 + 1 - (C - len))], es + sv - e[it]);
+      }
 #pragma unroll
-        for (int t = 0; t < 2 * (it + 1); ++t) {
-          if (DT == 0 && t == 2) {
-            O[it] *= __builtin_amdgcn_ldexpf(1.0f, e - e1);
-            e = e1;
-          }
-          O[it] = mfma<DT>(vf[t], p8(0, it, t), O[it]);
-          O[it] = mfma<DT>(vf[t], p8(1, it, t), O[it]);
+      for (int t = 0; t < T; ++t) {
+        if (DT == 0 && t == 2) {
+          O[IT - 1] *= __builtin_amdgcn_ldexpf(1.0f, e[IT - 1] - e1);
+          e[IT - 1] = e1;
         }
-        const float up = __builtin_amdgcn_ldexpf(a.scale, e);
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+          for (int it = t / 2; it < IT; ++it) O[it] = mfma<DT>(vf[t], p8(half, it, t), O[it]);
+      }
+      if constexpr (DT == 0) s_max = largest();
+#pragma unroll
+      for (int it = 0; it < IT; ++it) {
+        const float up = __builtin_amdgcn_ldexpf(a.scale, e[it]);
         const int row = 32 * it + l32 - (C - len);
         // a lane pair (l, l + 32) holds value dims 8 q + 0 .. 3 and 4 .. 7 of a token; it trades two q's halves for 16-byte stores
         uint16_t* o = static_cast<uint16_t*>(a.out) + (int64_t)(pos + row) * a.o_t + h * a.o_h + 32 * wv + 8 * g;
