@@ -306,20 +306,25 @@ __global__ __launch_bounds__(2 * D, 2) void chunk_kernel(Args a) {
 
   // ---- chunk loads through descriptors of the chunk's rows: the padding in front reads as zeros ----
   const int lc = tid % (D / 8), lr = tid / (D / 8);
-  const uint32_t qs = 2 * (uint32_t)a.q_t, ks = 2 * (uint32_t)a.k_t, vs = 2 * (uint32_t)a.v_t;  // row strides in bytes
+  const uint32_t qs = 2 * (uint32_t)a.q_t, ks = 2 * (uint32_t)a.k_t, vs = 2 * (uint32_t)a.v_t, os = 2 * (uint32_t)a.o_t;  // row strides in bytes
   const uint32_t q_off = lr * qs + 16 * lc, k_off = lr * ks + 16 * lc, v_off = lr * vs + 16 * lc;
   u32x4_t rq[T], rk[T], rv[T];
+  rsrc_t q_rows, k_rows, v_rows;
+  auto aim = [&](int from, int len) {
+    q_rows = make_rsrc(static_cast<const uint16_t*>(a.q) + (int64_t)from * a.q_t + h * a.q_h, (len - 1) * qs + 2 * D);
+    k_rows = make_rsrc(static_cast<const uint16_t*>(a.k) + (int64_t)from * a.k_t + hk * a.k_h, (len - 1) * ks + 2 * D);
+    v_rows = make_rsrc(static_cast<const uint16_t*>(a.v) + (int64_t)from * a.v_t + hk * a.v_h, (len - 1) * vs + 2 * D);
+  };
+  auto load_part = [&](int i, int len) {
+    const uint32_t row = 16u * i - (uint32_t)(C - len);  // (a row before the first wraps to an offset past the end)
+    rk[i] = bload128(k_rows, k_off + row * ks);
+    rv[i] = bload128(v_rows, v_off + row * vs);
+    if constexpr (OUT) rq[i] = bload128(q_rows, q_off + row * qs);
+  };
   auto load = [&](int from, int len) {
-    const rsrc_t q = make_rsrc(static_cast<const uint16_t*>(a.q) + (int64_t)from * a.q_t + h * a.q_h, (len - 1) * qs + 2 * D);
-    const rsrc_t k = make_rsrc(static_cast<const uint16_t*>(a.k) + (int64_t)from * a.k_t + hk * a.k_h, (len - 1) * ks + 2 * D);
-    const rsrc_t v = make_rsrc(static_cast<const uint16_t*>(a.v) + (int64_t)from * a.v_t + hk * a.v_h, (len - 1) * vs + 2 * D);
+    aim(from, len);
 #pragma unroll
-    for (int i = 0; i < T; ++i) {
-      const uint32_t row = 16u * i - (uint32_t)(C - len);  // (a row before the first wraps to an offset past the end)
-      if constexpr (OUT) rq[i] = bload128(q, q_off + row * qs);
-      rk[i] = bload128(k, k_off + row * ks);
-      rv[i] = bload128(v, v_off + row * vs);
-    }
+    for (int i = 0; i < T; ++i) load_part(i, len);
   };
   int single_until = pos;
   int len = min(C, end - pos);
@@ -380,50 +385,46 @@ __global__ __launch_bounds__(2 * D, 2) void chunk_kernel(Args a) {
 
   int sv = 0;  // S is kept times 2^-sv, which brings v's largest value near 2^10 (fp16)
   bool first_chunk = true;
-  // the largest finite |S| of the wave (magnitudes as integers: fmaxf would quiet every operand first)
-  auto largest = [&]() {
-    auto of = [&](bool finite) {
-      uint32_t m = 0;
-#pragma unroll
-      for (int mt = 0; mt < KT; ++mt)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const float v = S[mt][r];  // (a copy: bit_cast of a vector's element reads element 0)
-          const uint32_t x = __builtin_bit_cast(uint32_t, v) & 0x7FFFFFFFu;
-          m = max(m, finite && x >= 0x7F800000u ? 0u : x);
-        }
-      auto wider = [&](float y) { m = max(m, __builtin_bit_cast(uint32_t, y)); };
-      auto f = [&]() { return __builtin_bit_cast(float, m); };
-      wider(xor_partner<1>(f()));
-      wider(xor_partner<2>(f()));
-      wider(xor_partner<4>(f()));
-      wider(xor_partner<8>(f()));
-      const auto x = __builtin_amdgcn_permlane16_swap(m, m, false, false);
-      m = max((uint32_t)x[0], (uint32_t)x[1]);
-      const auto y = __builtin_amdgcn_permlane32_swap(m, m, false, false);
-      return (uint32_t)uniform((int)max((uint32_t)y[0], (uint32_t)y[1]));
-    };
-    uint32_t m = of(false);
-    if (m >= 0x7F800000u) m = of(true);
-    return __builtin_bit_cast(float, m);
-  };
   // the wave's score tile: (0, 0), (1, 1) and (1, 0) by wave; waves without one make one that is not read
   const int my_at = IT == 1 ? (wv == 0 ? 0 : 3) : (NW == 2 ? 2 * wv : (wv < 3 ? wv : 3));
   const int my_it = IT == 1 ? (wv == 0 ? 0 : 1) : (my_at == 1 || my_at == 2), my_jt = IT == 1 ? 0 : (my_at == 1 || my_at == 3);
   // (vmcnt 0: with the state's loads still counted as outstanding at the loop's head, the compiler waits for the
   // loop's own loads where it overwrites registers that held the state's)
   __builtin_amdgcn_s_waitcnt(0x0F70);
-  float s_max = 0.0f;
-  if constexpr (OUT && DT == 0) s_max = largest();
+  // A bound of the wave's finite |S|: the largest at first, then the largest
+  // that a chunk's halves had, decayed, and what the chunk can have added.
+  float s_bound = 0.0f;
+  if constexpr (OUT && DT == 0) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int mt = 0; mt < KT; ++mt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float v = S[mt][r];  // (a copy: bit_cast of a vector's element reads element 0)
+        const uint32_t x = __builtin_bit_cast(uint32_t, v) & 0x7FFFFFFFu;
+        m = max(m, x < 0x7F800000u ? x : 0u);
+      }
+    auto wider = [&](float y) { m = max(m, __builtin_bit_cast(uint32_t, y)); };
+    auto f = [&]() { return __builtin_bit_cast(float, m); };
+    wider(xor_partner<1>(f()));
+    wider(xor_partner<2>(f()));
+    wider(xor_partner<4>(f()));
+    wider(xor_partner<8>(f()));
+    const auto x = __builtin_amdgcn_permlane16_swap(m, m, false, false);
+    m = max((uint32_t)x[0], (uint32_t)x[1]);
+    const auto y = __builtin_amdgcn_permlane32_swap(m, m, false, false);
+    s_bound = __builtin_bit_cast(float, uniform((int)max((uint32_t)y[0], (uint32_t)y[1])));
+  }
   while (pos < end) {
     // ---- stage ----
-    uint32_t mv = 0;
+    uint32_t mv = 0, mk = 0;
 #pragma unroll
     for (int i = 0; i < T; ++i) {
       const int row = lr + 16 * i;
-      if constexpr (OUT || DT == 0) {
 #pragma unroll
-        for (int w = 0; w < 4; ++w) mv = pk_max(mv, rv[i][w] & 0x7FFF7FFFu);
+      for (int w = 0; w < 4; ++w) {
+        if constexpr (OUT || DT == 0) mv = pk_max(mv, rv[i][w] & 0x7FFF7FFFu);
+        if constexpr (OUT && DT == 0) mk = pk_max(mk, rk[i][w] & 0x7FFF7FFFu);
       }
       if constexpr (OUT) {
         char* q = lds + row * QP + 32 * (lc / 2) + 8 * (lc % 2);
@@ -434,15 +435,18 @@ __global__ __launch_bounds__(2 * D, 2) void chunk_kernel(Args a) {
       *reinterpret_cast<u32x4_t*>(lds + VO + row * KP + 16 * lc) = rv[i];
     }
     if constexpr (OUT || DT == 0) {
-      mv = wave_pk_max(pk_max(mv, mv >> 16));
+      mv = wave_pk_max((pk_max(mv, mv >> 16) & 0xFFFFu) | pk_max(mk, mk << 16) & 0xFFFF0000u);
       if (lane == 0) *reinterpret_cast<uint32_t*>(lds + MO + 4 * wv) = mv;
     }
     __syncthreads();
+    float kv_max = 0.0f;  // what the chunk can add to a value of S
     if constexpr (OUT || DT == 0) {
       uint32_t m = 0;
 #pragma unroll
       for (int w = 0; w < NW; ++w) m = pk_max(m, *reinterpret_cast<const uint32_t*>(lds + MO + 4 * w));
-      m = (uint32_t)uniform((int)m) & 0xFFFFu;
+      m = (uint32_t)uniform((int)m);
+      if constexpr (OUT && DT == 0) kv_max = (float)C * magnitude(m >> 16) * magnitude(m & 0xFFFFu);
+      m &= 0xFFFFu;
       if (OUT && len > 1 && m >= (DT == 0 ? 0x7C00u : 0x7F80u)) {
         single_until = pos + len;
         len = 1;
@@ -457,7 +461,7 @@ __global__ __launch_bounds__(2 * D, 2) void chunk_kernel(Args a) {
           const int now = excess(vmax, -100) + 5;
 #pragma unroll
           for (int mt = 0; mt < KT; ++mt) S[mt] = S[mt] * pow2(sv) * pow2(-now);
-          s_max = s_max * pow2(sv) * pow2(-now);
+          s_bound = s_bound * pow2(sv) * pow2(-now);
           sv = now;
           first_chunk = false;
           for (int n = tid; n < C; n += NT) left[n] = pw[C - 1 - n] * pow2(-sv);
@@ -467,11 +471,13 @@ __global__ __launch_bounds__(2 * D, 2) void chunk_kernel(Args a) {
     }
     const int next = pos + len;
     const int next_len = next < single_until ? 1 : min(C, end - next);
-    if (next < end) load(next, next_len);
+    const bool more = next < end;
+    aim(more ? next : pos, more ? next_len : len);
 
     u32x4_t vf[T];  // the wave's columns of v, 8 tokens a lane
     float16_t O[IT] = {}, P = {};
-    const int es = DT == 0 ? excess(s_max, -100) : 0;
+    const int es = DT == 0 ? excess(s_bound, -100) : 0;
+    uint32_t hi_max = 0;
     const float lambda_n = pw[len];
     float down = 1.0f;
     // A tile of the scores (rows j: key tokens, columns i), done in three
@@ -528,42 +534,54 @@ __global__ __launch_bounds__(2 * D, 2) void chunk_kernel(Args a) {
           split2<DT>(S[s / 2][8 * (s % 2) + 2 * p], s_down, S[s / 2][8 * (s % 2) + 2 * p + 1], s_down, x, y);
           hi[s % 2][p] = x;
           lo[s % 2][p] = y;
+          if constexpr (DT == 0) hi_max = pk_max(hi_max, x & 0x7FFF7FFFu);
         }
       };
       // one step's reads and halves ahead, and S's decay behind, in the shadow of the step's MFMAs
+      u32x4_t kp[2];
 #pragma unroll
       for (int it = 0; it < IT; ++it) qf[0][it] = q8(it, 0);
+      kp[0] = k8(my_jt, 0);
       halves(0);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int s = 0; s < 2 * KT; ++s) {
-        const u32x4_t kp = k8(my_jt, s), qp = q8(my_it, s);
+        u32x4_t qp = qf[s % 2][0];
+        if constexpr (IT == 2) {
+#pragma unroll
+          for (int w = 0; w < 4; ++w) qp[w] = my_it ? qf[s % 2][1][w] : qf[s % 2][0][w];
+        }
         if (s + 1 < 2 * KT) {
 #pragma unroll
           for (int it = 0; it < IT; ++it) qf[(s + 1) % 2][it] = q8(it, s + 1);
+          kp[(s + 1) % 2] = k8(my_jt, s + 1);
           halves(s + 1);
+        } else {
+#pragma unroll
+          for (int t = 0; t < T; ++t) vf[t] = col8(VO, t, 32 * wv);
         }
         if (s % 2) S[s / 2] *= lambda_n;
 #pragma unroll
         for (int it = 0; it < IT; ++it) O[it] = mfma<DT>(hi[s % 2], qf[s % 2][it], O[it]);
 #pragma unroll
         for (int it = 0; it < IT; ++it) O[it] = mfma<DT>(lo[s % 2], qf[s % 2][it], O[it]);
-        P = mfma<DT>(kp, qp, P);
-        __builtin_amdgcn_sched_group_barrier(0x100, IT + 3, 0);
+        P = mfma<DT>(kp[s % 2], qp, P);
+        if (s + 1 < 2 * KT) __builtin_amdgcn_sched_group_barrier(0x100, IT + 2, 0);
+        else __builtin_amdgcn_sched_group_barrier(0x100, 2 * T, 0);
 #pragma unroll
         for (int n = 0; n < 2 * IT + 1; ++n) {
           __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-          __builtin_amdgcn_sched_group_barrier(0x002, IT == 2 ? 8 : 12, 0);
+          __builtin_amdgcn_sched_group_barrier(0x002, IT == 2 ? 9 : 14, 0);
         }
         __builtin_amdgcn_sched_barrier(0);
       }
     } else {
 #pragma unroll
       for (int mt = 0; mt < KT; ++mt) S[mt] *= lambda_n;
-    }
 #pragma unroll
-    for (int t = 0; t < T; ++t) vf[t] = col8(VO, t, 32 * wv);
-    // ---- S <- lambda^n S (done) + k^T (decayed v), and the tile's exchange ----
+      for (int t = 0; t < T; ++t) vf[t] = col8(VO, t, 32 * wv);
+    }
+    // ---- S <- lambda^n S (done) + k^T (decayed v), the tile's exchange, and the next chunk's loads ----
     if (++applied == 16) {
       applied = 0;
 #pragma unroll
@@ -590,9 +608,13 @@ __global__ __launch_bounds__(2 * D, 2) void chunk_kernel(Args a) {
     decayed(0);
     if constexpr (OUT) masked(P, my_it == my_jt, my_at);
     __builtin_amdgcn_sched_barrier(0);
+    // (without a next chunk the descriptors are the present one's: the loads come to nothing, but their number is known)
 #pragma unroll
     for (int n = 0; n < N; ++n) {
       const int t = n / KN, m0 = n % KN * KB;
+#pragma unroll
+      for (int i = 0; i < T; ++i)
+        if (i * N / T == n) load_part(i, next_len);
       if (n + 1 < N) {
 #pragma unroll
         for (int m = 0; m < KB; ++m) kf[(n + 1) % 2][m] = col8(KO, (n + 1) / KN, 32 * ((n + 1) % KN * KB + m));
@@ -612,12 +634,14 @@ __global__ __launch_bounds__(2 * D, 2) void chunk_kernel(Args a) {
       for (int m = 0; m < 2 * KB; ++m) {
         __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
         __builtin_amdgcn_sched_group_barrier(0x002, 8, 0);
+        __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
       }
       __builtin_amdgcn_sched_barrier(0);
     }
     if constexpr (OUT) {
       __syncthreads();
       // ---- times the tokens' decay, + v^T P^T ----
+      const rsrc_t out_rows = make_rsrc(static_cast<uint16_t*>(a.out) + (int64_t)pos * a.o_t + h * a.o_h, (len - 1) * os + 2 * D);
       int e[IT], e1 = 0;  // the scores' exponents: of a row's first tile, and of its diagonal tile behind it
 #pragma unroll
       for (int it = 0; it < IT; ++it) {
@@ -640,21 +664,22 @@ __global__ __launch_bounds__(2 * D, 2) void chunk_kernel(Args a) {
 #pragma unroll
           for (int it = t / 2; it < IT; ++it) O[it] = mfma<DT>(vf[t], p8(half, it, t), O[it]);
       }
-      if constexpr (DT == 0) s_max = largest();
+      if constexpr (DT == 0) {
+        hi_max = wave_pk_max(pk_max(hi_max, hi_max >> 16));
+        s_bound = magnitude((uint32_t)uniform((int)hi_max) & 0xFFFFu) * pow2(es) * lambda_n + kv_max * pow2(-sv);
+      }
 #pragma unroll
       for (int it = 0; it < IT; ++it) {
         const float up = __builtin_amdgcn_ldexpf(a.scale, e[it]);
-        const int row = 32 * it + l32 - (C - len);
         // a lane pair (l, l + 32) holds value dims 8 q + 0 .. 3 and 4 .. 7 of a token; it trades two q's halves for 16-byte stores
-        uint16_t* o = static_cast<uint16_t*>(a.out) + (int64_t)(pos + row) * a.o_t + h * a.o_h + 32 * wv + 8 * g;
+        const uint32_t o = (uint32_t)(32 * it + l32 - (C - len)) * os + 2 * (32 * wv + 8 * g);  // (padding: past the end)
 #pragma unroll
         for (int q = 0; q < 4; q += 2) {
           const auto x = __builtin_amdgcn_permlane32_swap(pack2<DT>(O[it][4 * q] * up, O[it][4 * q + 1] * up),
                                                           pack2<DT>(O[it][4 * q + 4] * up, O[it][4 * q + 5] * up), false, false);
           const auto y = __builtin_amdgcn_permlane32_swap(pack2<DT>(O[it][4 * q + 2] * up, O[it][4 * q + 3] * up),
                                                           pack2<DT>(O[it][4 * q + 6] * up, O[it][4 * q + 7] * up), false, false);
-          if (row >= 0)
-            *reinterpret_cast<u32x4_t*>(o + 8 * q) = u32x4_t{(uint32_t)x[0], (uint32_t)y[0], (uint32_t)x[1], (uint32_t)y[1]};
+          bstore128(u32x4_t{(uint32_t)x[0], (uint32_t)y[0], (uint32_t)x[1], (uint32_t)y[1]}, out_rows, o + 16 * q);
         }
       }
     }
