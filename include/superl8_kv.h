@@ -586,7 +586,7 @@ int s8kv_append_rope_k8v3(const void* q, int num_q_heads, int64_t q_stride_t, in
  * on one workspace race.
  * _decode: one token per sequence.
  */
-int64_t s8kv_linear_attn_workspace_size(int batch, int num_q_heads, int head_dim, int max_seqlen);
+int64_t s8kv_linear_attn_workspace_size(int batch, int num_q_heads, int head_dim, int64_t num_tokens, int max_seqlen);
 int s8kv_linear_attn_varlen(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k, int64_t k_stride_t,
                             int64_t k_stride_h, const void* v, int64_t v_stride_t, int64_t v_stride_h,
                             int64_t num_tokens, int num_q_heads, int num_kv_heads, int head_dim, int dtype,

@@ -185,7 +185,7 @@ SIGNATURES: dict[str, tuple] = {
         _c_void_p, _i64, _i64, _c_void_p, _i64, _i64,
         _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i32, _i64, _i32, _c_void_p,
     ]),
-    "s8kv_linear_attn_workspace_size": (_i64, [_i32, _i32, _i32, _i32]),
+    "s8kv_linear_attn_workspace_size": (_i64, [_i32, _i32, _i32, _i64, _i32]),
     "s8kv_linear_attn_varlen": (_i32, [
         _c_void_p, _i64, _i64, _c_void_p, _i64, _i64, _c_void_p, _i64, _i64, _i64, _i32, _i32, _i32, _i32,
         _c_void_p, _c_void_p, _i64, _i64, _c_void_p, _c_void_p, _c_void_p, _i32, _i32, _f32,

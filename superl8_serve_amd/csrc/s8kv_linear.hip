@@ -330,21 +330,6 @@ __global__ __launch_bounds__(2 * D, 2) void chunk_kernel(Args a) {
   int len = min(C, end - pos);
   if (pos < end) load(pos, len);
 
-  // ---- powers of lambda ----
-  float* const pw = reinterpret_cast<float*>(lds + LO);
-  float* const left = reinterpret_cast<float*>(lds + LR);
-  const double gd = (double)a.log_decay[h];
-  if (tid < 32) pw[tid - 32] = 1.0f;  // (what masked scores meet)
-  for (int n = tid; n <= C; n += NT) {
-    const float x = (float)exp(n ? gd * n : 0.0);
-    pw[n] = x;
-    if (n < C) left[C - 1 - n] = x;
-  }
-  // lambda^C, of whose fp32 value's rounding 16 applications are made good at a time
-  const Factor lambda_c(gd * C);
-  const float drift = lambda_c.hi > 0.0f ? 16.0f * lambda_c.lo / lambda_c.hi : 0.0f;
-  int applied = 0;
-
   // ---- the state's columns 32 wv + l32: register r of tile mt is key dim 32 mt + 8 (r / 4) + 4 g + r % 4 ----
   const int64_t s_at = 4 * g * D + 32 * wv + l32;
   float* const pool = a.state + slot * a.state_slot + (int64_t)h * D * D + s_at;
@@ -362,6 +347,21 @@ __global__ __launch_bounds__(2 * D, 2) void chunk_kernel(Args a) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) S[mt][r] = src[(32 * mt + 8 * (r / 4) + r % 4) * D];
   }
+
+  // ---- powers of lambda ----
+  float* const pw = reinterpret_cast<float*>(lds + LO);
+  float* const left = reinterpret_cast<float*>(lds + LR);
+  const double gd = (double)a.log_decay[h];
+  if (tid < 32) pw[tid - 32] = 1.0f;  // (what masked scores meet)
+  for (int n = tid; n <= C; n += NT) {
+    const float x = (float)exp(n ? gd * n : 0.0);
+    pw[n] = x;
+    if (n < C) left[C - 1 - n] = x;
+  }
+  // lambda^C is applied as its fp32 value, whose rounding is made good 16 applications at a time
+  const Factor lambda_c(gd * C);
+  const float drift = lambda_c.hi > 0.0f ? 16.0f * lambda_c.lo / lambda_c.hi : 0.0f;
+  int applied = 0;
 
   // operands: 8 values of a row (row l32 of the tile) and of a column (by
   // transposed reads).  q rows hold their dims in the order of S's
@@ -737,27 +737,30 @@ static int launch_chunks(Args& a, const char* what, hipStream_t stream) {
   return check_launch(what);
 }
 
-// Segments a sequence of max_seqlen tokens is split into (1: not split).
-static int plan_segments(int batch, int heads, int head_dim, int max_seqlen) {
-  const int64_t pairs = (int64_t)batch * heads, want = 2 * device_cus();
-  if (pairs == 0 || pairs >= want / 2) return 1;
-  int64_t n = want / pairs;
-  const int64_t most = max_seqlen / 512;
-  n = n < most ? n : most;
-  return n < 1 ? 1 : (int)n;
+// Tokens of the segments that long sequences are split into (0: no split).
+// A CU works off one (sequence, head) alone at nearly the rate of two side by
+// side, so a batch is even enough while its longest sequence is no longer than
+// the tokens a CU has to do altogether; else segments of half of those, two a
+// CU.  Splitting reads k and v of all but the last segments a second time.
+constexpr int kLeastSegment = 256;
+static int segment_tokens(int64_t tokens, int heads, int head_dim, int max_seqlen) {
+  const int64_t share = tokens * heads * head_dim / (128 * (int64_t)device_cus());
+  if (max_seqlen <= share + share / 5 || max_seqlen <= 2 * kLeastSegment) return 0;
+  const int64_t seg = share / 2 > kLeastSegment ? share / 2 : kLeastSegment;
+  const int64_t n = (max_seqlen + seg - 1) / seg;
+  return (int)((max_seqlen + n - 1) / n + 63) / 64 * 64;
 }
-static int64_t parts_bytes(int batch, int heads, int head_dim, int num_seg) {
-  return num_seg <= 1 ? 0 : (int64_t)batch * heads * num_seg * head_dim * head_dim * 4;
-}
-
 template <int DT>
-static int launch_varlen(Args& a, int head_dim, const char* what, hipStream_t stream) {
+static int launch_varlen(Args& a, int head_dim, int max_seqlen, const char* what, hipStream_t stream) {
   // (a chunk's rows have 32-bit offsets, one bit of them for the rows that are not there)
   auto rows = [](const void* p, int64_t t, int64_t h) {
     return (uintptr_t)p % 16 == 0 && t % 8 == 0 && h % 8 == 0 && t >= 0 && t < (1 << 24);
   };
   if (!(rows(a.q, a.q_t, a.q_h) && rows(a.k, a.k_t, a.k_h) && rows(a.v, a.v_t, a.v_h) && rows(a.out, a.o_t, a.o_h)))
     return launch<DT>(a, head_dim, what, stream);
+  // a few tokens: the recurrence reads and writes the state at once (head_dim 128, 32 sequences x 32 heads: 6 tokens
+  // 27.7 us against the chunk's 34.2, 8 tokens 32.0 / 33.9, 12 tokens 39.5 / 34.2; head_dim 64: 12 tokens 15.7 / 18.5)
+  if ((int64_t)max_seqlen * head_dim <= 768) return launch<DT>(a, head_dim, what, stream);
   switch (head_dim) {
     case 32: return launch_chunks<32, DT>(a, what, stream);
     case 64: return launch_chunks<64, DT>(a, what, stream);
@@ -815,21 +818,22 @@ extern "C" int s8kv_linear_attn_varlen(const void* q, int64_t q_stride_t, int64_
   S8KV_REQUIRE(max_seqlen >= 0, S8KV_ERR_INVALID, "%s: max_seqlen < 0", what);
   a.cu = cu_seqlens;
   if (batch == 0 || (num_tokens == 0 && !reset)) return S8KV_OK;
-  const int num_seg = linear::plan_segments(batch, num_q_heads, head_dim, max_seqlen);
-  if (num_seg > 1 && workspace && (uintptr_t)workspace % 16 == 0 &&
-      workspace_bytes >= linear::parts_bytes(batch, num_q_heads, head_dim, num_seg)) {
-    a.num_seg = num_seg;
-    a.seg_len = (max_seqlen / num_seg + 64) / 64 * 64;
+  const int seg = linear::segment_tokens(num_tokens, num_q_heads, head_dim, max_seqlen);
+  if (seg && workspace && (uintptr_t)workspace % 16 == 0 &&
+      workspace_bytes >= s8kv_linear_attn_workspace_size(batch, num_q_heads, head_dim, num_tokens, max_seqlen)) {
+    a.num_seg = (max_seqlen + seg - 1) / seg;
+    a.seg_len = seg;
     a.parts = static_cast<float*>(workspace);
   }
-  return dtype == 0 ? linear::launch_varlen<0>(a, head_dim, what, (hipStream_t)stream)
-                    : linear::launch_varlen<1>(a, head_dim, what, (hipStream_t)stream);
+  return dtype == 0 ? linear::launch_varlen<0>(a, head_dim, max_seqlen, what, (hipStream_t)stream)
+                    : linear::launch_varlen<1>(a, head_dim, max_seqlen, what, (hipStream_t)stream);
 }
 
-extern "C" int64_t s8kv_linear_attn_workspace_size(int batch, int num_q_heads, int head_dim, int max_seqlen) {
-  if (batch <= 0 || num_q_heads <= 0 || head_dim <= 0 || max_seqlen <= 0) return 0;
-  return linear::parts_bytes(batch, num_q_heads, head_dim,
-                             linear::plan_segments(batch, num_q_heads, head_dim, max_seqlen));
+extern "C" int64_t s8kv_linear_attn_workspace_size(int batch, int num_q_heads, int head_dim, int64_t num_tokens,
+                                                   int max_seqlen) {
+  if (batch <= 0 || num_q_heads <= 0 || head_dim <= 0 || num_tokens <= 0 || max_seqlen <= 0) return 0;
+  const int seg = linear::segment_tokens(num_tokens, num_q_heads, head_dim, max_seqlen);
+  return seg ? (int64_t)batch * num_q_heads * ((max_seqlen + seg - 1) / seg) * head_dim * head_dim * 4 : 0;
 }
 
 extern "C" int s8kv_linear_attn_decode(const void* q, int64_t q_stride_b, int64_t q_stride_h, const void* k,

@@ -1240,7 +1240,7 @@ def linear_attn_varlen(q, k, v, log_decay, state, cu_seqlens, max_seqlen, *, sta
     if b == 0:
         return out.zero_()
     lib = _lib.load()
-    ws_bytes = int(lib.s8kv_linear_attn_workspace_size(b, hq, d, max_seqlen))
+    ws_bytes = int(lib.s8kv_linear_attn_workspace_size(b, hq, d, t, max_seqlen))
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
     rc = _launch(q.device, lib.s8kv_linear_attn_varlen, q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0),
                  k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), t, hq, k.shape[1], d, code, *args,
