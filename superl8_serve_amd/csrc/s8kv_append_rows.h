@@ -199,8 +199,10 @@ __device__ __forceinline__ float lloyd3_threshold(float a, float b) {
 // lloyd3_search_ok) lloyd3_search's three tests as compares against the
 // thresholds thr[j] = T_j, else the sequential scan.  Parts 2g and 2g + 1
 // (lanes l and l ^ 1) hold elements 32g .. 32g + 31: each builds 16 bits of
-// the three bit-plane words 3g + b, and the even part stores them.
-template <int D, class VOut, class NOut>
+// the three bit-plane words 3g + b, and the even part stores them.  THR false:
+// no thresholds (finding them takes a workgroup longer than a row or two):
+// lloyd3_search's own tests.
+template <int D, bool THR = true, class VOut, class NOut>
 __device__ __forceinline__ void rows_lloydmax3_store(const float (&x)[16], bool live, int li, bool search,
                                                      const float (&cb)[8], const float (&thr)[8], const VOut& vout,
                                                      const NOut& nout) {
@@ -230,10 +232,15 @@ __device__ __forceinline__ void rows_lloydmax3_store(const float (&x)[16], bool 
   if (search) {
 #pragma unroll
     for (int i = 15; i >= 0; --i) {
-      const bool b2 = u[i] >= thr[4];
-      const bool b1 = u[i] >= (b2 ? thr[6] : thr[2]);
-      const float t_hi = b2 ? thr[7] : thr[3], t_lo = b2 ? thr[5] : thr[1];
-      const bool b0 = u[i] >= (b1 ? t_hi : t_lo);
+      bool b2, b1, b0;
+      if constexpr (THR) {
+        b2 = u[i] >= thr[4];
+        b1 = u[i] >= (b2 ? thr[6] : thr[2]);
+        const float t_hi = b2 ? thr[7] : thr[3], t_lo = b2 ? thr[5] : thr[1];
+        b0 = u[i] >= (b1 ? t_hi : t_lo);
+      } else {
+        lloyd3_search(u[i], cb, b2, b1, b0);
+      }
       pw[0] = shift_in_bit(pw[0], b0);
       pw[1] = shift_in_bit(pw[1], b1);
       pw[2] = shift_in_bit(pw[2], b2);

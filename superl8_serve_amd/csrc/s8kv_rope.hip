@@ -107,30 +107,24 @@ __device__ __forceinline__ void expand(const Raw<DT>& r, float (&x)[16]) {
     for (int j = 0; j < 16; ++j) x[j] = __builtin_bit_cast(float, (uint32_t)r.w[j / 4][j % 4]);
   }
 }
+typedef float float2_t __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 template <int DT>
 __device__ __forceinline__ void store_part(char* p, const float (&x)[16]) {
   u32x4_t* o = reinterpret_cast<u32x4_t*>(p);
-  if constexpr (DT == 0) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      half8_t h;
+  for (int j = 0; j < (DT == 2 ? 4 : 2); ++j) {
+    u32x4_t w;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) h[i] = (_Float16)pin(x[8 * j + i]);
-      o[j] = __builtin_bit_cast(u32x4_t, h);
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (DT == 0)
+        w[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(float2_t{x[8 * j + 2 * i], x[8 * j + 2 * i + 1]}, half2_t));
+      else if constexpr (DT == 1)
+        w[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(float2_t{x[8 * j + 2 * i], x[8 * j + 2 * i + 1]}, bf16x2_t));
+      else
+        w[i] = __builtin_bit_cast(uint32_t, x[4 * j + i]);
     }
-  } else if constexpr (DT == 1) {
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      bf16x8_t h;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) h[i] = (__bf16)pin(x[8 * j + i]);
-      o[j] = __builtin_bit_cast(u32x4_t, h);
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      o[j] = u32x4_t{__builtin_bit_cast(uint32_t, x[4 * j]), __builtin_bit_cast(uint32_t, x[4 * j + 1]),
-                     __builtin_bit_cast(uint32_t, x[4 * j + 2]), __builtin_bit_cast(uint32_t, x[4 * j + 3])};
+    o[j] = w;
   }
 }
 
@@ -145,89 +139,78 @@ __device__ __forceinline__ int axis_of(const Args& a, int pair) {
 }
 __device__ __forceinline__ int position(const Args& a, int axis, int64_t t) { return a.pos[axis * a.pos_stride + t]; }
 
-// cos and signed sin (-s for a pair's first value, +s for its second) of the
-// lane's 16 values; 1 and 0 are not used for the dims past R (`turns` false).
+// The cosines and sines of a wave's tokens, through the wave's part of LDS:
+// each pair's two table values are read once a token, whatever the axes, and
+// then by every lane that holds one of the pair's values (read straight from
+// the table, 16 + 16 values a lane, the gathers of three axes took a third of
+// the kernel's time).  Per token: c of the R/2 pairs, -s, s.
+template <int D>
+constexpr int kAngleFloats = 3 * (D / 2) * RowsLayout<D>::RPW;  // of a wave (at most RPW tokens)
 template <int D>
 struct Angles {
-  float c[16], s[16];
-  bool turns;
-  __device__ __forceinline__ void load(const Args& a, int64_t t, bool live, int li) {
+  float c[16], s[16];  // s: -s for a pair's first value, +s for its second
+  bool turns;          // false: the lane's dims are past R
+  static __device__ __forceinline__ void gather(const Args& a, int64_t t0, int tokens, int lane, float* lds) {
+    const int half = a.rot >> 1;
+    for (int k = 0; k < tokens; ++k) {
+      const int64_t t = t0 + k;
+      if (t >= a.tokens) break;
+      for (int pair = lane; pair < half; pair += 64) {
+        const float* row = table_row(a, position(a, a.axes == 1 ? 0 : axis_of(a, pair), t));
+        const float nan = __builtin_nanf("");
+        const float c = row ? row[pair] : nan, s = row ? row[half + pair] : nan;
+        float* o = lds + k * 3 * half + pair;
+        o[0] = c;
+        o[half] = -s;
+        o[2 * half] = s;
+      }
+    }
+    // (the wave's LDS instructions run in order; the fence keeps the compiler's order)
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  }
+  // the lane's values; `lds`: its token's
+  __device__ __forceinline__ void take(const Args& a, const float* lds, int li) {
     const int half = a.rot >> 1;
     turns = 16 * li < a.rot;
-    const float nan = __builtin_nanf("");
+    if (!turns) return;
+    if (a.adjacent) {
+      const float4_t* cp = reinterpret_cast<const float4_t*>(lds + 8 * li);
+      const float4_t* np = reinterpret_cast<const float4_t*>(lds + half + 8 * li);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) c[i] = s[i] = nan;
-    if (!live || !turns) return;
-    if (a.axes == 1) {
-      const float* row = table_row(a, position(a, 0, t));
-      if (!row) return;
-      if (a.adjacent) {
-        const float4_t* cp = reinterpret_cast<const float4_t*>(row + 8 * li);
-        const float4_t* sp = reinterpret_cast<const float4_t*>(row + half + 8 * li);
+      for (int j = 0; j < 2; ++j) {
+        const float4_t cv = cp[j], nv = np[j];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const float4_t cv = cp[j], sv = sp[j];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            c[8 * j + 2 * i] = c[8 * j + 2 * i + 1] = cv[i];
-            s[8 * j + 2 * i] = -sv[i];
-            s[8 * j + 2 * i + 1] = sv[i];
-          }
-        }
-      } else if (a.partner) {
-        const bool second = (li & a.partner) != 0;
-        const int p0 = 16 * (li & (a.partner - 1));
-        const float4_t* cp = reinterpret_cast<const float4_t*>(row + p0);
-        const float4_t* sp = reinterpret_cast<const float4_t*>(row + half + p0);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float4_t cv = cp[j], sv = sp[j];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            c[4 * j + i] = cv[i];
-            s[4 * j + i] = second ? sv[i] : -sv[i];
-          }
-        }
-      } else {  // R = 16: pairs (i, i + 8) of part 0
-        const float4_t* cp = reinterpret_cast<const float4_t*>(row);
-        const float4_t* sp = reinterpret_cast<const float4_t*>(row + 8);
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const float4_t cv = cp[j], sv = sp[j];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            c[4 * j + i] = c[8 + 4 * j + i] = cv[i];
-            s[4 * j + i] = -sv[i];
-            s[8 + 4 * j + i] = sv[i];
-          }
+        for (int i = 0; i < 4; ++i) {
+          c[8 * j + 2 * i] = c[8 * j + 2 * i + 1] = cv[i];
+          s[8 * j + 2 * i] = nv[i];
+          s[8 * j + 2 * i + 1] = -nv[i];
         }
       }
-      return;
-    }
-    // several axes: the pairs' rows differ
-    const float* rows[4];
+    } else if (a.partner) {
+      const int p0 = 16 * (li & (a.partner - 1));
+      const float4_t* cp = reinterpret_cast<const float4_t*>(lds + p0);
+      const float4_t* sp = reinterpret_cast<const float4_t*>(lds + ((li & a.partner) ? 2 * half : half) + p0);
 #pragma unroll
-    for (int x = 0; x < 4; ++x) rows[x] = x < a.axes ? table_row(a, position(a, x, t)) : nullptr;
+      for (int j = 0; j < 4; ++j) {
+        const float4_t cv = cp[j], sv = sp[j];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      int pair;
-      bool second;
-      if (a.adjacent) {
-        pair = 8 * li + i / 2;
-        second = i & 1;
-      } else if (a.partner) {
-        pair = 16 * (li & (a.partner - 1)) + i;
-        second = (li & a.partner) != 0;
-      } else {
-        pair = i & 7;
-        second = i >= 8;
+        for (int i = 0; i < 4; ++i) {
+          c[4 * j + i] = cv[i];
+          s[4 * j + i] = sv[i];
+        }
       }
-      const int ax = axis_of(a, pair);
-      const float* row = ax < 2 ? (ax == 0 ? rows[0] : rows[1]) : (ax == 2 ? rows[2] : rows[3]);
-      if (row) {
-        c[i] = row[pair];
-        const float sv = row[half + pair];
-        s[i] = second ? sv : -sv;
+    } else {  // R = 16: pairs (i, i + 8) of part 0
+      const float4_t* cp = reinterpret_cast<const float4_t*>(lds);
+      const float4_t* np = reinterpret_cast<const float4_t*>(lds + half);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float4_t cv = cp[j], nv = np[j];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          c[4 * j + i] = c[8 + 4 * j + i] = cv[i];
+          s[4 * j + i] = nv[i];
+          s[8 + 4 * j + i] = -nv[i];
+        }
       }
     }
   }
@@ -252,10 +235,15 @@ struct Angles {
 #pragma unroll
       for (int i = 0; i < 16; ++i) y[i] = x[i ^ 8];
     }
+    if (a.rot == D) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const float r = x[i] * c[i] + y[i] * s[i];
-      x[i] = turns ? r : x[i];
+      for (int i = 0; i < 16; ++i) x[i] = x[i] * c[i] + y[i] * s[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float r = x[i] * c[i] + y[i] * s[i];
+        x[i] = turns ? r : x[i];
+      }
     }
   }
 };
@@ -264,7 +252,7 @@ struct Angles {
 // (in-lane, then across the row's lanes), mean, + eps, correctly rounded
 // square root and reciprocal.
 template <int D>
-__device__ __forceinline__ void normalise(const Args& a, const void* weight, float (&x)[16], int li) {
+__device__ __forceinline__ void normalise(const Args& a, const float (&w)[16], float (&x)[16]) {
   constexpr int LPR = RowsLayout<D>::LPR;
   float s[16];
 #pragma unroll
@@ -281,7 +269,7 @@ __device__ __forceinline__ void normalise(const Args& a, const void* weight, flo
   if constexpr (LPR > 8) t = t + xor_partner<8>(t);
   const float r = 1.0f / __builtin_sqrtf(t * a.inv_d + a.eps);
 #pragma unroll
-  for (int i = 0; i < 16; ++i) x[i] = x[i] * r * load_any(weight, 16 * li + i, a.norm_dtype);
+  for (int i = 0; i < 16; ++i) x[i] = x[i] * r * w[i];
 }
 
 // A token's cache row of KV head h, or false: a negative slot or one outside
@@ -294,44 +282,70 @@ __device__ __forceinline__ bool cache_row(const Args& a, int64_t t, int h, uint6
   return slot >= 0 && (int64_t)blk < a.num_blocks;
 }
 
-// modes: 0 q and k out, 1 int8 cache, 2 K8V3 cache
+// modes: 0 q and k out, 1 int8 cache, 2 K8V3 cache.  A wave takes the heads of
+// its token (or tokens, where there are fewer heads than rows a wave) in
+// iterations of RPW rows, q's first, then k's, then v's, with the next
+// iteration's row in flight: its lanes' angles are fetched once.
 template <int D, int DT, int MODE>
 __global__ __launch_bounds__(64 * kWaves) void rope_rows_kernel(Args a) {
   using L = RowsLayout<D>;
-  const int lane = threadIdx.x & 63;
+  __shared__ __attribute__((aligned(16))) float lds[kWaves][kAngleFloats<D>];
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int li = L::part(lane);
   const int chunks = (a.iters + a.per_wave - 1) / a.per_wave;
-  const int64_t wave = (int64_t)blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int64_t wave = (int64_t)blockIdx.x * kWaves + wv;
   const int64_t group = wave / chunks;
   const int it0 = (int)(wave - group * chunks) * a.per_wave;
   const int it1 = min(a.iters, it0 + a.per_wave);
-  const int hpi = 1 << a.hpi_log2;
-  const int64_t t = group * (L::RPW >> a.hpi_log2) + (L::row(lane) >> a.hpi_log2);
+  const int hpi = 1 << a.hpi_log2, tokens = L::RPW >> a.hpi_log2;
+  const int64_t t = group * tokens + (L::row(lane) >> a.hpi_log2);
   const int sub = L::row(lane) & (hpi - 1);
   const bool here = t < a.tokens;
   const int nq = (a.q.heads + hpi - 1) >> a.hpi_log2, nk = (a.k.heads + hpi - 1) >> a.hpi_log2;
 
-  Angles<D> angles;
-  if (it0 < nq + nk) angles.load(a, t, here, li);
   const RowsHadamard<D> hadamard(li, a.rot_norm);
-  float cb[8], thr[8];
+  float cb[8], w[16];
+  bool search = false;
   if constexpr (MODE == 2) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) cb[i] = thr[i] = a.v_codebook[i];
+    for (int i = 0; i < 8; ++i) cb[i] = a.v_codebook[i];
+    search = lloyd3_search_ok(cb);
   }
+  auto kind_of = [&](int it) { return it < nq ? 0 : (it < nq + nk ? 1 : 2); };
+  auto head_of = [&](int it, int kind) { return ((it - (kind == 0 ? 0 : (kind == 1 ? nq : nq + nk))) << a.hpi_log2) + sub; };
+  auto fetch = [&](int it) {
+    const int kind = kind_of(it), h = head_of(it, kind);
+    const Rows& rows = kind == 0 ? a.q : (kind == 1 ? a.k : a.v);
+    Raw<DT> raw{};
+    if (here && h < rows.heads) raw = load_raw<DT>(rows.p + (t * rows.st + h * rows.sh + 16 * li) * kBytes<DT>);
+    return raw;
+  };
+  Raw<DT> next{};
+  if (it0 < it1) next = fetch(it0);
+  Angles<D> angles;
+  if (it0 < nq + nk) {
+    Angles<D>::gather(a, group * tokens, tokens, lane, lds[wv]);
+    if (here) angles.take(a, lds[wv] + (L::row(lane) >> a.hpi_log2) * 3 * (a.rot >> 1), li);
+  }
+  int w_kind = -1;  // whose norm weights w holds
 
 #pragma unroll 1
   for (int it = it0; it < it1; ++it) {
-    const int kind = it < nq ? 0 : (it < nq + nk ? 1 : 2);
+    const int kind = kind_of(it), h = head_of(it, kind);
     const Rows& rows = kind == 0 ? a.q : (kind == 1 ? a.k : a.v);
-    const int h = ((kind == 0 ? it : (kind == 1 ? it - nq : it - nq - nk)) << a.hpi_log2) + sub;
     const bool live = here && h < rows.heads;
-    Raw<DT> raw{};
-    if (live) raw = load_raw<DT>(rows.p + (t * rows.st + h * rows.sh + 16 * li) * kBytes<DT>);
     float x[16];
-    expand<DT>(raw, x);
+    expand<DT>(next, x);
+    if (it + 1 < it1) next = fetch(it + 1);
     if (kind < 2) {
-      if (rows.norm) normalise<D>(a, rows.norm, x, li);
+      if (rows.norm) {
+        if (kind != w_kind) {
+          w_kind = kind;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) w[i] = load_any(rows.norm, 16 * li + i, a.norm_dtype);
+        }
+        normalise<D>(a, w, x);
+      }
       angles.turn(a, x);
       char* out = kind == 0 ? a.q_out : a.k_out;
       if (live && out) {
@@ -352,8 +366,8 @@ __global__ __launch_bounds__(64 * kWaves) void rope_rows_kernel(Args a) {
       } else if constexpr (MODE == 1) {
         rows_rtn_store<D>(x, write, li, PtrOut{a.v_cache + row * D}, PtrOut{reinterpret_cast<char*>(a.v_scale + row)});
       } else {
-        rows_lloydmax3_store<D>(x, write, li, false, cb, thr, PtrOut{a.v_cache + row * (D / 32 * 3 * 4)},
-                                PtrOut{reinterpret_cast<char*>(a.v_scale + row * (D / 128))});
+        rows_lloydmax3_store<D, false>(x, write, li, search, cb, cb, PtrOut{a.v_cache + row * (D / 32 * 3 * 4)},
+                                       PtrOut{reinterpret_cast<char*>(a.v_scale + row * (D / 128))});
       }
     }
   }

@@ -1007,11 +1007,16 @@ def _axis_map(sections: tuple, interleaved: bool, half: int):
 
 
 _PAIRINGS = {"half": 0, "adjacent": 1}
+_LINEAR_DTYPES = {torch.float16: 0, torch.bfloat16: 1}  # (of the rotating writes and the linear attention)
 
 
-def _rope_args(q, k, positions, cos_sin, sections, interleaved, pairing, q_norm, k_norm, eps):
-    """The checks and the C arguments that the rotation and the rotating
-    writes share: (tokens, rotation arguments, what must outlive the call)."""
+def _norm_ok(w, d: int, dev: int) -> bool:
+    return w is None or (w.get_device() == dev and w.shape == (d,) and w.dtype in _ROT_DTYPES and w.is_contiguous())
+
+
+def _rope_checked(q, k, positions, cos_sin, sections, interleaved, pairing, q_norm, k_norm):
+    """Every check of what the rotation takes beside q and k, one by one;
+    returns the tensors as the kernels read them."""
     dev, t, d = q.device, q.shape[0], q.shape[2]
     _require(k is None or k.shape[2] == d, lambda: f"k head_dim {k.shape[2]} != q head_dim {d}")
     _on_gpu("positions", positions, torch.int32, dev)
@@ -1020,20 +1025,17 @@ def _rope_args(q, k, positions, cos_sin, sections, interleaved, pairing, q_norm,
              "cos_sin must be a contiguous [max_positions, rot_dim] tensor")
     rot = cos_sin.shape[1]
     _require(0 < rot <= d and rot % 2 == 0, lambda: f"cos_sin's rot_dim {rot} must be even and at most head_dim {d}")
-    if pairing not in _PAIRINGS:
-        raise ValueError(f"pairing must be 'half' or 'adjacent', got {pairing!r}")
+    _require(pairing in _PAIRINGS, lambda: f"pairing must be 'half' or 'adjacent', got {pairing!r}")
     if sections is None:
         _require(not interleaved, "interleaved needs sections")
         _require(tuple(positions.shape) in ((t,), (1, t)), lambda: f"positions must be [{t}], got {tuple(positions.shape)}")
-        axes, amap = 1, None
     else:
-        amap = _axis_map(tuple(sections), bool(interleaved), rot // 2)
         axes = len(sections)
+        _axis_map(tuple(sections), bool(interleaved), rot // 2)
         _require(tuple(positions.shape) == (axes, t),
                  lambda: f"positions must be [{axes}, {t}], got {tuple(positions.shape)}")
     if t and positions.stride(-1) != 1:
         positions = positions.contiguous()
-    norm_dtype = 0
     norms = [None, None]
     for i, (name, w) in enumerate((("q_norm", q_norm), ("k_norm", k_norm))):
         if w is None:
@@ -1041,13 +1043,36 @@ def _rope_args(q, k, positions, cos_sin, sections, interleaved, pairing, q_norm,
         _on_gpu(name, w, None, dev)
         _require(w.dtype in _ROT_DTYPES, lambda: f"{name}: dtype {w.dtype} not in fp16 / bf16 / fp32", TypeError)
         _require(w.dim() == 1 and w.shape[0] == d, lambda: f"{name} must be [{d}], got {tuple(w.shape)}")
-        norms[i] = w if w.is_contiguous() else w.contiguous()
-        norm_dtype = _ROT_DTYPES[w.dtype]
-    _require(norms[0] is None or norms[1] is None or norms[0].dtype == norms[1].dtype, "q_norm and k_norm differ in dtype")
-    args = (positions.data_ptr(), axes, positions.stride(0) if positions.dim() == 2 else 0, amap, cos_sin.data_ptr(),
-            cos_sin.shape[0], rot, _PAIRINGS[pairing], None if norms[0] is None else norms[0].data_ptr(),
-            None if norms[1] is None else norms[1].data_ptr(), norm_dtype, eps)
-    return args, (positions, norms)
+        norms[i] = w.contiguous()
+    _require(None in norms or norms[0].dtype == norms[1].dtype, "q_norm and k_norm differ in dtype")
+    return positions, cos_sin, norms[0], norms[1]
+
+
+def _rope_args(q, k, positions, cos_sin, sections, interleaved, pairing, q_norm, k_norm, eps):
+    """The C arguments that the rotation and the rotating writes share, and
+    what must outlive the call.  (The usual call is recognised by one test;
+    the checks one by one take twice an op's other host time.)"""
+    dev = q.get_device()
+    t, _, d = q.shape
+    if not (type(positions) is type(cos_sin) is torch.Tensor and positions.get_device() == cos_sin.get_device() == dev
+            and positions.dtype is torch.int32 and cos_sin.dtype is torch.float32 and sections is None
+            and not interleaved and positions.shape == (t,) and positions.is_contiguous() and cos_sin.dim() == 2
+            and cos_sin.is_contiguous() and cos_sin.shape[0] > 0 and 0 < cos_sin.shape[1] <= d
+            and cos_sin.shape[1] % 2 == 0 and pairing in _PAIRINGS and (k is None or k.shape[2] == d)
+            and type(q_norm) is type(k_norm) and _norm_ok(q_norm, d, dev) and _norm_ok(k_norm, d, dev)
+            and (q_norm is None or q_norm.dtype is k_norm.dtype)):
+        positions, cos_sin, q_norm, k_norm = _rope_checked(q, k, positions, cos_sin, sections, interleaved, pairing,
+                                                           q_norm, k_norm)
+    rows, rot = cos_sin.shape
+    if sections is None:
+        axes, amap = 1, None
+    else:
+        axes, amap = len(sections), _axis_map(tuple(sections), bool(interleaved), rot // 2)
+    norm = q_norm if q_norm is not None else k_norm
+    args = (positions.data_ptr(), axes, positions.stride(0) if axes > 1 else 0, amap, cos_sin.data_ptr(), rows, rot,
+            _PAIRINGS[pairing], None if q_norm is None else q_norm.data_ptr(), None if k_norm is None else k_norm.data_ptr(),
+            0 if norm is None else _ROT_DTYPES[norm.dtype], eps)
+    return args, (positions, q_norm, k_norm)
 
 
 def _rope_out(out, name: str, like: torch.Tensor, dtype) -> torch.Tensor:
@@ -1094,7 +1119,7 @@ def rope(q, k, positions, cos_sin, *, sections=None, interleaved: bool = False, 
         k_out = _rope_out(k_out, "k_out", k, dtype)
         ks = (src_k.data_ptr(), k.shape[1], src_k.stride(0), src_k.stride(1))
         kos = (k_out.data_ptr(), k_out.stride(0), k_out.stride(1))
-    if t and hq:
+    if t:
         rc = _launch(dev, _lib.load().s8kv_rope, src_q.data_ptr(), hq, src_q.stride(0), src_q.stride(1), *ks, t, d,
                      _ROT_DTYPES[dtype], *args, q_out.data_ptr(), q_out.stride(0), q_out.stride(1), *kos, _stream(q))
         _lib.check(rc, "rope")
@@ -1103,29 +1128,36 @@ def rope(q, k, positions, cos_sin, *, sections=None, interleaved: bool = False, 
 
 def _rope_write(what, entry, q, k, v, positions, cos_sin, k_cache, k_scale, slot_mapping, tail, sections, interleaved,
                 pairing, q_norm, k_norm, eps, q_out, k_out):
-    _require(q.dtype in (torch.float16, torch.bfloat16), lambda: f"{what}: dtype {q.dtype} not in fp16 / bf16", TypeError)
     dev, dtype = q.device, q.dtype
-    _on_gpu("k_scale", k_scale, torch.float32, dev)
-    _on_gpu("slot_mapping", slot_mapping, torch.int32, dev)
-    n, hkv, bs, d = _cache_geometry(k_cache)
-    _require(tuple(k_scale.shape) == (n, hkv, bs) and k_scale.is_contiguous(), "k_scale must be [N, Hkv, bs] contiguous")
-    _require(q.dim() == 3 and q.shape[2] == d, lambda: f"q must be [tokens, heads, {d}], got {tuple(q.shape)}")
-    t, hq, _ = q.shape
-    src_q = _heads_view(q, "q", t, dtype, dev)
-    k, v = _heads_view(k, "k", t, dtype, dev), _heads_view(v, "v", t, dtype, dev)
-    _require(k.shape[1:] == (hkv, d) and v.shape == k.shape, lambda: f"k and v must be [{t}, {hkv}, {d}]")
-    _require(slot_mapping.dim() == 1 and slot_mapping.shape[0] == t, lambda: f"slot_mapping must be [{t}]")
-    slot_mapping = slot_mapping.contiguous()
-    args, keep = _rope_args(src_q, k, positions, cos_sin, sections, interleaved, pairing, q_norm, k_norm, eps)
+    n, hkv, bs, d = k_cache.shape
+    t = slot_mapping.shape[0] if slot_mapping.dim() == 1 else -1
+    if not (dtype in _LINEAR_DTYPES and k.dtype is v.dtype is dtype and k.device == v.device == dev
+            and slot_mapping.device == k_scale.device == dev and slot_mapping.dtype is torch.int32
+            and k_scale.dtype is torch.float32 and k_scale.shape == (n, hkv, bs) and k_scale.is_contiguous()
+            and q.dim() == 3 and k.shape == v.shape == (t, hkv, d) and q.shape[0] == t and q.shape[2] == d
+            and q.stride(2) == k.stride(2) == v.stride(2) == 1 and slot_mapping.is_contiguous()):
+        _require(dtype in _LINEAR_DTYPES, lambda: f"{what}: dtype {dtype} not in fp16 / bf16", TypeError)
+        _on_gpu("k_scale", k_scale, torch.float32, dev)
+        _on_gpu("slot_mapping", slot_mapping, torch.int32, dev)
+        _require(tuple(k_scale.shape) == (n, hkv, bs) and k_scale.is_contiguous(), "k_scale must be [N, Hkv, bs] contiguous")
+        _require(q.dim() == 3 and q.shape[2] == d, lambda: f"q must be [tokens, heads, {d}], got {tuple(q.shape)}")
+        t = q.shape[0]
+        q = _heads_view(q, "q", t, dtype, dev)
+        k, v = _heads_view(k, "k", t, dtype, dev), _heads_view(v, "v", t, dtype, dev)
+        _require(k.shape[1:] == (hkv, d) and v.shape == k.shape, lambda: f"k and v must be [{t}, {hkv}, {d}]")
+        _require(slot_mapping.dim() == 1 and slot_mapping.shape[0] == t, lambda: f"slot_mapping must be [{t}]")
+        slot_mapping = slot_mapping.contiguous()
+    hq = q.shape[1]
+    args, keep = _rope_args(q, k, positions, cos_sin, sections, interleaved, pairing, q_norm, k_norm, eps)
     q_out = _rope_out(q_out, "q_out", q, torch.float16)
     if k_out is None:
         kos = (None, 0, 0)
     else:
         k_out = _rope_out(k_out, "k_out", k, torch.float16)
         kos = (k_out.data_ptr(), k_out.stride(0), k_out.stride(1))
-    if t and hq:
-        rc = _launch(dev, entry, src_q.data_ptr(), hq, src_q.stride(0), src_q.stride(1), k.data_ptr(), v.data_ptr(), hkv,
-                     k.stride(0), k.stride(1), v.stride(0), v.stride(1), t, d, _ROT_DTYPES[dtype], *args,
+    if t:
+        rc = _launch(dev, entry, q.data_ptr(), hq, q.stride(0), q.stride(1), k.data_ptr(), v.data_ptr(), hkv,
+                     k.stride(0), k.stride(1), v.stride(0), v.stride(1), t, d, _LINEAR_DTYPES[dtype], *args,
                      q_out.data_ptr(), q_out.stride(0), q_out.stride(1), *kos, slot_mapping.data_ptr(),
                      k_cache.data_ptr(), k_scale.data_ptr(), *tail, n, bs, _stream(q))
         _lib.check(rc, what)
@@ -1147,6 +1179,7 @@ def quantize_kv_write_paged_rope(q, k, v, positions, cos_sin, k_cache, k_scale, 
     _on_gpu("k_cache", k_cache, torch.int8, q.device)
     _on_gpu("v_cache", v_cache, torch.int8, q.device)
     _on_gpu("v_scale", v_scale, torch.float32, q.device)
+    _cache_geometry(k_cache)
     _require(v_cache.shape == k_cache.shape and v_cache.is_contiguous(), "v_cache must match k_cache")
     _require(v_scale.shape == k_scale.shape and v_scale.is_contiguous(), "v_scale must be [N, Hkv, bs] contiguous")
     return _rope_write("quantize_kv_write_paged_rope", _lib.load().s8kv_append_rope_int8, q, k, v, positions, cos_sin,
@@ -1184,12 +1217,11 @@ def quantize_kv_write_paged_k8v3_rope(q, k, v, positions, cos_sin, k_cache, k_sc
 # ---------------------------------------------------------------------------
 
 
-def _linear_args(q, k, v, log_decay, state, state_slots, reset, batch):
-    """Checks shared by the two forms: (q, k, v, dtype code, what follows the
-    dtype in the C arguments, tensors that must outlive the call)."""
-    _on_gpu("q", q)
+def _linear_checked(q, k, v, log_decay, state, state_slots, reset, batch):
+    """Every check of the linear attention's arguments, one by one; returns
+    them as the kernels read them."""
     dev, dtype = q.device, q.dtype
-    _require(dtype in (torch.float16, torch.bfloat16), lambda: f"linear_attn: dtype {dtype} not in fp16 / bf16", TypeError)
+    _require(dtype in _LINEAR_DTYPES, lambda: f"linear_attn: dtype {dtype} not in fp16 / bf16", TypeError)
     _require(q.dim() == 3, lambda: f"q must be [tokens, heads, head_dim], got {tuple(q.shape)}")
     t, hq, d = q.shape
     q, k, v = _heads_view(q, "q", t, dtype, dev), _heads_view(k, "k", t, dtype, dev), _heads_view(v, "v", t, dtype, dev)
@@ -1212,9 +1244,28 @@ def _linear_args(q, k, v, log_decay, state, state_slots, reset, batch):
         _require(reset.dtype in (torch.bool, torch.uint8), lambda: f"reset: dtype {reset.dtype} not in bool / uint8", TypeError)
         _require(reset.dim() == 1 and reset.shape[0] == batch, lambda: f"reset must be [{batch}]")
         reset = reset.contiguous()
-    args = (log_decay.data_ptr(), state.data_ptr(), state.stride(0) if state.shape[0] > 1 else hq * d * d, state.shape[0],
-            None if state_slots is None else state_slots.data_ptr(), None if reset is None else reset.data_ptr())
-    return q, k, v, _ROT_DTYPES[dtype], args, (log_decay, state_slots, reset)
+    return q, k, v, log_decay, state_slots, reset
+
+
+def _linear_args(q, k, v, log_decay, state, state_slots, reset, batch):
+    """(q, k, v, the C arguments from the dtype on, what must outlive the
+    call).  The usual call is recognised by one test."""
+    dev, dtype = q.device, q.dtype
+    if not (type(log_decay) is type(state) is torch.Tensor and dtype in _LINEAR_DTYPES and k.dtype is v.dtype is dtype
+            and k.device == v.device == log_decay.device == state.device == dev
+            and log_decay.dtype is state.dtype is torch.float32 and q.dim() == k.dim() == 3 and k.shape == v.shape
+            and q.shape[0] == k.shape[0] and q.shape[2] == k.shape[2] and k.shape[1] > 0
+            and q.shape[1] % k.shape[1] == 0 and q.stride(2) == k.stride(2) == v.stride(2) == 1
+            and log_decay.shape == q.shape[1:2] and log_decay.is_contiguous() and state.dim() == 4
+            and state.is_contiguous() and state.shape[1:] == (q.shape[1], q.shape[2], q.shape[2]) and reset is None
+            and (state_slots is None or (state_slots.dtype is torch.int32 and state_slots.device == dev
+                                         and state_slots.shape == (batch,) and state_slots.is_contiguous()))):
+        q, k, v, log_decay, state_slots, reset = _linear_checked(q, k, v, log_decay, state, state_slots, reset, batch)
+    _, hq, d = q.shape
+    slots = state.shape[0]
+    args = (_LINEAR_DTYPES[dtype], log_decay.data_ptr(), state.data_ptr(), state.stride(0) if slots > 1 else hq * d * d,
+            slots, None if state_slots is None else state_slots.data_ptr(), None if reset is None else reset.data_ptr())
+    return q, k, v, args, (log_decay, state_slots, reset)
 
 
 def linear_attn_varlen(q, k, v, log_decay, state, cu_seqlens, max_seqlen, *, state_slots=None, reset=None, scale):
@@ -1234,7 +1285,7 @@ def linear_attn_varlen(q, k, v, log_decay, state, cu_seqlens, max_seqlen, *, sta
     _require(cu_seqlens.dim() == 1 and cu_seqlens.numel() >= 1, "cu_seqlens must be [B + 1]")
     cu_seqlens, b, max_seqlen = cu_seqlens.contiguous(), cu_seqlens.numel() - 1, int(max_seqlen)
     _require(max_seqlen >= 0, "max_seqlen must be >= 0")
-    q, k, v, code, args, keep = _linear_args(q, k, v, log_decay, state, state_slots, reset, b)
+    q, k, v, args, keep = _linear_args(q, k, v, log_decay, state, state_slots, reset, b)
     t, hq, d = q.shape
     out = torch.empty((t, hq, d), dtype=q.dtype, device=q.device)
     if b == 0:
@@ -1243,7 +1294,7 @@ def linear_attn_varlen(q, k, v, log_decay, state, cu_seqlens, max_seqlen, *, sta
     ws_bytes = int(lib.s8kv_linear_attn_workspace_size(b, hq, d, t, max_seqlen))
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
     rc = _launch(q.device, lib.s8kv_linear_attn_varlen, q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0),
-                 k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), t, hq, k.shape[1], d, code, *args,
+                 k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), t, hq, k.shape[1], d, *args,
                  cu_seqlens.data_ptr(), b, max_seqlen, scale, out.data_ptr(), hq * d, d,
                  None if ws is None else ws.data_ptr(), ws_bytes, _stream(q))
     _lib.check(rc, "linear_attn_varlen")
@@ -1255,13 +1306,13 @@ def linear_attn_decode(q, k, v, log_decay, state, *, state_slots=None, reset=Non
     ``k``, ``v`` ``[B, Hkv, D]``; returns ``[B, Hq, D]``."""
     _on_gpu("q", q)
     b = q.shape[0] if q.dim() else 0
-    q, k, v, code, args, keep = _linear_args(q, k, v, log_decay, state, state_slots, reset, b)
+    q, k, v, args, keep = _linear_args(q, k, v, log_decay, state, state_slots, reset, b)
     hq, d = q.shape[1:]
     out = torch.empty((b, hq, d), dtype=q.dtype, device=q.device)
     if b == 0:
         return out
     rc = _launch(q.device, _lib.load().s8kv_linear_attn_decode, q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(),
-                 k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), b, hq, k.shape[1], d, code, *args,
+                 k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), b, hq, k.shape[1], d, *args,
                  scale, out.data_ptr(), hq * d, d, _stream(q))
     _lib.check(rc, "linear_attn_decode")
     return out
