@@ -59,6 +59,7 @@ struct Args {
   int64_t max_pos;
   int rot;
   int adjacent;
+  int pairs_log2;  // lanes a token's pairs take: the power of two from R / 2 on, 64 at most
   int partner;  // half pairing: parts between a pair's values (1, 2, 4, 8), 0: both on one lane
   int norm_dtype;
   float eps, inv_d;
@@ -109,22 +110,37 @@ __device__ __forceinline__ void expand(const Raw<DT>& r, float (&x)[16]) {
 }
 typedef float float2_t __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+// Stores the lane's 16 values at p.  16-bit types: lanes l and l ^ 1 (parts
+// 2 g and 2 g + 1) trade halves first, so that each of the two stores writes
+// whole 32-byte pieces (own halves in two stores made twice the write requests).
 template <int DT>
-__device__ __forceinline__ void store_part(char* p, const float (&x)[16]) {
-  u32x4_t* o = reinterpret_cast<u32x4_t*>(p);
+__device__ __forceinline__ void store_part(char* p, const float (&x)[16], int lane) {
+  if constexpr (DT == 2) {
+    u32x4_t* o = reinterpret_cast<u32x4_t*>(p);
 #pragma unroll
-  for (int j = 0; j < (DT == 2 ? 4 : 2); ++j) {
-    u32x4_t w;
+    for (int j = 0; j < 4; ++j)
+      o[j] = u32x4_t{__builtin_bit_cast(uint32_t, x[4 * j]), __builtin_bit_cast(uint32_t, x[4 * j + 1]),
+                     __builtin_bit_cast(uint32_t, x[4 * j + 2]), __builtin_bit_cast(uint32_t, x[4 * j + 3])};
+  } else {
+    u32x4_t w[2];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float2_t v = {x[2 * i], x[2 * i + 1]};
+      if constexpr (DT == 0) w[i / 4][i % 4] = __builtin_bit_cast(uint32_t, __builtin_convertvector(v, half2_t));
+      else w[i / 4][i % 4] = __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2_t));
+    }
+    const bool odd = lane & 1;
+    u32x4_t first, second;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      if constexpr (DT == 0)
-        w[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(float2_t{x[8 * j + 2 * i], x[8 * j + 2 * i + 1]}, half2_t));
-      else if constexpr (DT == 1)
-        w[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(float2_t{x[8 * j + 2 * i], x[8 * j + 2 * i + 1]}, bf16x2_t));
-      else
-        w[i] = __builtin_bit_cast(uint32_t, x[4 * j + i]);
+      const uint32_t own0 = w[0][i], own1 = w[1][i];
+      const uint32_t got = (uint32_t)__builtin_amdgcn_mov_dpp((int)(odd ? own0 : own1), 0xB1, 0xF, 0xF, false);  // lane ^ 1
+      first[i] = odd ? got : own0;
+      second[i] = odd ? own1 : got;
     }
-    o[j] = w;
+    p -= odd ? 16 : 0;  // (an odd part begins 32 bytes on: its second 16 bytes of the pair's first 32)
+    *reinterpret_cast<u32x4_t*>(p) = first;
+    *reinterpret_cast<u32x4_t*>(p + 32) = second;
   }
 }
 
@@ -152,17 +168,34 @@ struct Angles {
   bool turns;          // false: the lane's dims are past R
   static __device__ __forceinline__ void gather(const Args& a, int64_t t0, int tokens, int lane, float* lds) {
     const int half = a.rot >> 1;
-    for (int k = 0; k < tokens; ++k) {
-      const int64_t t = t0 + k;
-      if (t >= a.tokens) break;
-      for (int pair = lane; pair < half; pair += 64) {
-        const float* row = table_row(a, position(a, a.axes == 1 ? 0 : axis_of(a, pair), t));
-        const float nan = __builtin_nanf("");
-        const float c = row ? row[pair] : nan, s = row ? row[half + pair] : nan;
-        float* o = lds + k * 3 * half + pair;
-        o[0] = c;
-        o[half] = -s;
-        o[2 * half] = s;
+    constexpr int U = 4;  // tokens whose two dependent loads are in flight together
+    const int at = lane >> a.pairs_log2, first = lane & ((1 << a.pairs_log2) - 1), step = 64 >> a.pairs_log2;
+    for (int pair = first; pair < half; pair += 64) {  // (more than 64 pairs: the whole wave on one token)
+      const int axis = a.axes == 1 ? 0 : axis_of(a, pair);
+      for (int k = at; k < tokens; k += U * step) {
+        const float* row[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int64_t t = t0 + k + u * step;
+          row[u] = k + u * step < tokens && t < a.tokens ? table_row(a, position(a, axis, t)) : nullptr;
+        }
+        float c[U], s[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          c[u] = s[u] = __builtin_nanf("");
+          if (row[u]) {
+            c[u] = row[u][pair];
+            s[u] = row[u][half + pair];
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if (k + u * step >= tokens) break;
+          float* o = lds + (k + u * step) * 3 * half + pair;
+          o[0] = c[u];
+          o[half] = -s[u];
+          o[2 * half] = s[u];
+        }
       }
     }
     // (the wave's LDS instructions run in order; the fence keeps the compiler's order)
@@ -252,7 +285,7 @@ struct Angles {
 // (in-lane, then across the row's lanes), mean, + eps, correctly rounded
 // square root and reciprocal.
 template <int D>
-__device__ __forceinline__ void normalise(const Args& a, const float (&w)[16], float (&x)[16]) {
+__device__ __forceinline__ void normalise(const Args& a, const float* w, float (&x)[16]) {
   constexpr int LPR = RowsLayout<D>::LPR;
   float s[16];
 #pragma unroll
@@ -269,7 +302,11 @@ __device__ __forceinline__ void normalise(const Args& a, const float (&w)[16], f
   if constexpr (LPR > 8) t = t + xor_partner<8>(t);
   const float r = 1.0f / __builtin_sqrtf(t * a.inv_d + a.eps);
 #pragma unroll
-  for (int i = 0; i < 16; ++i) x[i] = x[i] * r * w[i];
+  for (int j = 0; j < 4; ++j) {
+    const float4_t wv = reinterpret_cast<const float4_t*>(w)[j];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[4 * j + i] = x[4 * j + i] * r * wv[i];
+  }
 }
 
 // A token's cache row of KV head h, or false: a negative slot or one outside
@@ -303,8 +340,18 @@ __global__ __launch_bounds__(64 * kWaves) void rope_rows_kernel(Args a) {
   const bool here = t < a.tokens;
   const int nq = (a.q.heads + hpi - 1) >> a.hpi_log2, nk = (a.k.heads + hpi - 1) >> a.hpi_log2;
 
+  // the norm weights in fp32, once a workgroup
+  __shared__ __attribute__((aligned(16))) float norms[2][D];
+  if (a.q.norm || a.k.norm) {
+    for (int i = threadIdx.x; i < 2 * D; i += 64 * kWaves) {
+      const void* w = i < D ? a.q.norm : a.k.norm;
+      if (w) norms[i / D][i % D] = load_any(w, i % D, a.norm_dtype);
+    }
+    __syncthreads();
+  }
+
   const RowsHadamard<D> hadamard(li, a.rot_norm);
-  float cb[8], w[16];
+  float cb[8];
   bool search = false;
   if constexpr (MODE == 2) {
 #pragma unroll
@@ -312,46 +359,44 @@ __global__ __launch_bounds__(64 * kWaves) void rope_rows_kernel(Args a) {
     search = lloyd3_search_ok(cb);
   }
   auto kind_of = [&](int it) { return it < nq ? 0 : (it < nq + nk ? 1 : 2); };
-  auto head_of = [&](int it, int kind) { return ((it - (kind == 0 ? 0 : (kind == 1 ? nq : nq + nk))) << a.hpi_log2) + sub; };
+  auto first_head = [&](int it, int kind) { return (it - (kind == 0 ? 0 : (kind == 1 ? nq : nq + nk))) << a.hpi_log2; };
+  const char* const rows[3] = {a.q.p + (t * a.q.st + sub * a.q.sh + 16 * li) * kBytes<DT>,
+                               a.k.p + (t * a.k.st + sub * a.k.sh + 16 * li) * kBytes<DT>,
+                               MODE ? a.v.p + (t * a.v.st + sub * a.v.sh + 16 * li) * kBytes<DT> : nullptr};
   auto fetch = [&](int it) {
-    const int kind = kind_of(it), h = head_of(it, kind);
-    const Rows& rows = kind == 0 ? a.q : (kind == 1 ? a.k : a.v);
+    const int kind = kind_of(it), h = first_head(it, kind);
+    const int64_t sh = kind == 0 ? a.q.sh : (kind == 1 ? a.k.sh : a.v.sh);
+    const int heads = kind == 0 ? a.q.heads : (kind == 1 ? a.k.heads : a.v.heads);
+    const char* p = kind == 0 ? rows[0] : (kind == 1 ? rows[1] : rows[2]);
     Raw<DT> raw{};
-    if (here && h < rows.heads) raw = load_raw<DT>(rows.p + (t * rows.st + h * rows.sh + 16 * li) * kBytes<DT>);
+    if (here && h + sub < heads) raw = load_raw<DT>(p + h * sh * kBytes<DT>);
     return raw;
   };
-  Raw<DT> next{};
+  Raw<DT> next{}, after{};  // the rows of the next iteration, and of the one after it
   if (it0 < it1) next = fetch(it0);
+  if (it0 + 1 < it1) after = fetch(it0 + 1);
   Angles<D> angles;
   if (it0 < nq + nk) {
     Angles<D>::gather(a, group * tokens, tokens, lane, lds[wv]);
     if (here) angles.take(a, lds[wv] + (L::row(lane) >> a.hpi_log2) * 3 * (a.rot >> 1), li);
   }
-  int w_kind = -1;  // whose norm weights w holds
 
 #pragma unroll 1
   for (int it = it0; it < it1; ++it) {
-    const int kind = kind_of(it), h = head_of(it, kind);
-    const Rows& rows = kind == 0 ? a.q : (kind == 1 ? a.k : a.v);
-    const bool live = here && h < rows.heads;
+    const int kind = kind_of(it), h = first_head(it, kind) + sub;
+    const bool live = here && h < (kind == 0 ? a.q.heads : a.k.heads);
     float x[16];
     expand<DT>(next, x);
-    if (it + 1 < it1) next = fetch(it + 1);
+    next = after;
+    if (it + 2 < it1) after = fetch(it + 2);
     if (kind < 2) {
-      if (rows.norm) {
-        if (kind != w_kind) {
-          w_kind = kind;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) w[i] = load_any(rows.norm, 16 * li + i, a.norm_dtype);
-        }
-        normalise<D>(a, w, x);
-      }
+      if (kind == 0 ? a.q.norm : a.k.norm) normalise<D>(a, norms[kind] + 16 * li, x);
       angles.turn(a, x);
       char* out = kind == 0 ? a.q_out : a.k_out;
       if (live && out) {
         const int64_t off = kind == 0 ? t * a.qo_t + h * a.qo_h : t * a.ko_t + h * a.ko_h;
         constexpr int OT = MODE ? 0 : DT;  // the writing modes hand q and k on in fp16
-        store_part<OT>(out + (off + 16 * li) * kBytes<OT>, x);
+        store_part<OT>(out + (off + 16 * li) * kBytes<OT>, x, lane);
       }
     }
     if constexpr (MODE > 0) {
@@ -486,14 +531,15 @@ static bool aligned(const void* p, int64_t st, int64_t sh, int bytes) {
 template <int D, int DT, int MODE>
 static int launch(Args& a, const char* what, hipStream_t stream) {
   const int bytes = kBytes<DT>, obytes = MODE ? 2 : bytes;
-  const int parts = a.rot / 32;  // half pairing: parts between a pair's values
+  const int apart = a.rot / 32;  // half pairing: parts between a pair's values
   const bool rows = aligned(a.q.p, a.q.st, a.q.sh, bytes) && aligned(a.k.p, a.k.st, a.k.sh, bytes) &&
                     aligned(a.v.p, a.v.st, a.v.sh, bytes) && aligned(a.q_out, a.qo_t, a.qo_h, obytes) &&
                     aligned(a.k_out, a.ko_t, a.ko_h, obytes) && (uintptr_t)a.table % 16 == 0 && a.rot % 16 == 0 &&
-                    (a.adjacent || a.rot == 16 || (a.rot % 32 == 0 && is_pow2(parts)));
+                    (a.adjacent || a.rot == 16 || (a.rot % 32 == 0 && is_pow2(apart)));
   if (rows) {
     constexpr int RPW = RowsLayout<D>::RPW;
-    a.partner = a.adjacent || a.rot == 16 ? 0 : parts;
+    a.partner = a.adjacent || a.rot == 16 ? 0 : apart;
+    a.pairs_log2 = log2i(a.rot / 2 < 64 ? a.rot / 2 : 64);
     int fewest = a.q.heads;
     if (a.k.heads && a.k.heads < fewest) fewest = a.k.heads;
     a.hpi_log2 = 0;
@@ -501,9 +547,12 @@ static int launch(Args& a, const char* what, hipStream_t stream) {
     const int hpi = 1 << a.hpi_log2, tokens = RPW >> a.hpi_log2;
     a.iters = (a.q.heads + hpi - 1) / hpi + (a.k.heads + hpi - 1) / hpi + (a.v.heads + hpi - 1) / hpi;
     const int64_t groups = (a.tokens + tokens - 1) / tokens;
-    const int64_t want = (int64_t)device_cus() * 4 * 8;  // waves that the GPU holds
+    // as many waves as the GPU holds, each with an equal share of its tokens' iterations (a wave's start, the chain
+    // from the positions to the angles, takes as long as several of them)
+    const int64_t want = (int64_t)device_cus() * 16;
     const int64_t each = groups * a.iters / want;
-    a.per_wave = (int)(each < 1 ? 1 : (each > a.iters ? a.iters : each));
+    const int parts = (int)(each < 1 ? a.iters : (each > a.iters ? 1 : (a.iters + each - 1) / each));
+    a.per_wave = (a.iters + parts - 1) / parts;
     const int64_t waves = groups * ((a.iters + a.per_wave - 1) / a.per_wave);
     const int64_t grid = (waves + kWaves - 1) / kWaves;
     S8KV_REQUIRE(grid < (int64_t(1) << 31), S8KV_ERR_INVALID, "%s: too many tokens (%lld)", what, (long long)a.tokens);
