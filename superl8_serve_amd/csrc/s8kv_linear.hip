@@ -27,7 +27,7 @@ struct Args {
   float scale;
   // the chunked form: segments a sequence may have, their tokens, their states
   int num_seg, seg_len;
-  float* parts;  // [batch][heads][num_seg][D][D]
+  float* parts;  // [entries][heads][D][D], part_of
 };
 
 template <int DT>
@@ -149,11 +149,16 @@ static int launch_recurrent(const Args& a, const char* what, hipStream_t stream)
 
 template <int DT>
 static int launch(const Args& a, int head_dim, const char* what, hipStream_t stream) {
+  const bool few = (int64_t)a.batch * a.heads < device_cus();
   switch (head_dim) {
     case 32: return launch_recurrent<32, DT, 32>(a, what, stream);
     case 64: return launch_recurrent<64, DT, 64>(a, what, stream);
-    case 128: return launch_recurrent<128, DT, 128>(a, what, stream);
-    case 256: return launch_recurrent<256, DT, 64>(a, what, stream);
+    case 128:
+      if (few) return launch_recurrent<128, DT, 32>(a, what, stream);
+      return launch_recurrent<128, DT, 128>(a, what, stream);
+    case 256:
+      if (few) return launch_recurrent<256, DT, 32>(a, what, stream);
+      return launch_recurrent<256, DT, 64>(a, what, stream);
   }
   return S8KV_ERR_UNSUPPORTED;
 }
@@ -257,6 +262,11 @@ __device__ __forceinline__ int segments(const Args& a, int len) {
   return min(max((int)(((unsigned)len + a.seg_len - 1) / (unsigned)a.seg_len), 1), a.num_seg);
 }
 
+// The entry of a sequence's first segment in `parts`: its segments take at
+// most one more than its tokens fill, so sequences one behind the other get
+// entries of their own, tokens / seg_len + batch altogether.
+__device__ __forceinline__ int64_t part_of(const Args& a, int b, int first) { return first / a.seg_len + b; }
+
 // OUT: outputs (from the segments' start states, where a sequence has
 // several) and the final state.  Else a segment's own contribution to the
 // state, from zero, for scan_kernel.
@@ -333,7 +343,7 @@ __global__ __launch_bounds__(2 * D, 2) void chunk_kernel(Args a) {
   // ---- the state's columns 32 wv + l32: register r of tile mt is key dim 32 mt + 8 (r / 4) + 4 g + r % 4 ----
   const int64_t s_at = 4 * g * D + 32 * wv + l32;
   float* const pool = a.state + slot * a.state_slot + (int64_t)h * D * D + s_at;
-  float* const parts = a.parts + ((int64_t)b * a.heads + h) * a.num_seg * D * D + s_at;
+  float* const parts = a.parts + ((part_of(a, b, first_t) + seg) * a.heads + h) * D * D + s_at;
   float16_t S[KT];
   if (!OUT || (nseg == 1 && fresh)) {
 #pragma unroll
@@ -341,7 +351,7 @@ __global__ __launch_bounds__(2 * D, 2) void chunk_kernel(Args a) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) S[mt][r] = 0.0f;
   } else {
-    const float* src = nseg > 1 ? parts + (int64_t)seg * D * D : pool;
+    const float* src = nseg > 1 ? parts : pool;
 #pragma unroll
     for (int mt = 0; mt < KT; ++mt)
 #pragma unroll
@@ -688,7 +698,7 @@ __global__ __launch_bounds__(2 * D, 2) void chunk_kernel(Args a) {
     __syncthreads();
   }
   if (OUT && seg < nseg - 1) return;
-  float* dst = OUT ? pool : parts + (int64_t)(seg + 1) * D * D;
+  float* dst = OUT ? pool : parts + (int64_t)a.heads * D * D;  // (the next segment's start)
 #pragma unroll
   for (int mt = 0; mt < KT; ++mt)
 #pragma unroll
@@ -710,13 +720,13 @@ __global__ __launch_bounds__(256) void scan_kernel(Args a) {
   const int nseg = segments(a, last_t - first_t);
   if (nseg == 1 || slot < 0 || slot >= a.num_slots) return;
   const int64_t at = 1024 * tile + 4 * threadIdx.x;
-  float* p = a.parts + ((int64_t)b * a.heads + h) * a.num_seg * D * D + at;
+  float* p = a.parts + (part_of(a, b, first_t) * a.heads + h) * D * D + at;
   const Factor lambda((double)a.log_decay[h] * a.seg_len);
   float4_t s = {0, 0, 0, 0};
   if (!(a.reset && a.reset[b])) s = *reinterpret_cast<const float4_t*>(a.state + slot * a.state_slot + (int64_t)h * D * D + at);
   *reinterpret_cast<float4_t*>(p) = s;
   for (int i = 1; i < nseg; ++i) {
-    p += D * D;
+    p += (int64_t)a.heads * D * D;
     const float4_t x = *reinterpret_cast<const float4_t*>(p);
 #pragma unroll
     for (int c = 0; c < 4; ++c) s[c] = lambda(s[c]) + x[c];
@@ -744,6 +754,7 @@ static int launch_chunks(Args& a, const char* what, hipStream_t stream) {
 // CU.  Splitting reads k and v of all but the last segments a second time.
 constexpr int kLeastSegment = 256;
 static int segment_tokens(int64_t tokens, int heads, int head_dim, int max_seqlen) {
+  if (max_seqlen > tokens) max_seqlen = (int)tokens;  // (a graph's bucket, say)
   const int64_t share = tokens * heads * head_dim / (128 * (int64_t)device_cus());
   if (max_seqlen <= share + share / 5 || max_seqlen <= 2 * kLeastSegment) return 0;
   const int64_t seg = share / 2 > kLeastSegment ? share / 2 : kLeastSegment;
@@ -821,7 +832,8 @@ extern "C" int s8kv_linear_attn_varlen(const void* q, int64_t q_stride_t, int64_
   const int seg = linear::segment_tokens(num_tokens, num_q_heads, head_dim, max_seqlen);
   if (seg && workspace && (uintptr_t)workspace % 16 == 0 &&
       workspace_bytes >= s8kv_linear_attn_workspace_size(batch, num_q_heads, head_dim, num_tokens, max_seqlen)) {
-    a.num_seg = (max_seqlen + seg - 1) / seg;
+    const int longest = max_seqlen < num_tokens ? max_seqlen : (int)num_tokens;
+    a.num_seg = (longest + seg - 1) / seg;
     a.seg_len = seg;
     a.parts = static_cast<float*>(workspace);
   }
@@ -833,7 +845,7 @@ extern "C" int64_t s8kv_linear_attn_workspace_size(int batch, int num_q_heads, i
                                                    int max_seqlen) {
   if (batch <= 0 || num_q_heads <= 0 || head_dim <= 0 || num_tokens <= 0 || max_seqlen <= 0) return 0;
   const int seg = linear::segment_tokens(num_tokens, num_q_heads, head_dim, max_seqlen);
-  return seg ? (int64_t)batch * num_q_heads * ((max_seqlen + seg - 1) / seg) * head_dim * head_dim * 4 : 0;
+  return seg ? (num_tokens / seg + batch) * num_q_heads * head_dim * head_dim * 4 : 0;
 }
 
 extern "C" int s8kv_linear_attn_decode(const void* q, int64_t q_stride_b, int64_t q_stride_h, const void* k,

@@ -974,7 +974,7 @@ def gather_slots(tensors: Sequence[torch.Tensor], src_slots: Sequence[int], dst_
 def _launch(device: torch.device, entry, *args) -> int:
     """``entry(*args)`` with ``device`` current: a launch on the default stream
     (handle 0) goes to the current device, whatever the tensors' is."""
-    if device.index == torch._C._cuda_getDevice():
+    if device.index == torch._C._cuda_getDevice():  # (torch.cuda.current_device without its 0.5 us)
         return entry(*args)
     with torch.cuda.device(device):
         return entry(*args)
@@ -1077,7 +1077,7 @@ def _rope_args(q, k, positions, cos_sin, sections, interleaved, pairing, q_norm,
 
 def _rope_out(out, name: str, like: torch.Tensor, dtype) -> torch.Tensor:
     if out is None:
-        return torch.empty(like.shape, dtype=dtype, device=like.device)
+        return like.new_empty(like.shape, dtype=dtype)
     _on_gpu(name, out, dtype, like.device)
     _require(out.shape == like.shape and out.stride(2) == 1,
              lambda: f"{name} must be {tuple(like.shape)} with a unit stride on its last dim")
@@ -1102,13 +1102,15 @@ def rope(q, k, positions, cos_sin, *, sections=None, interleaved: bool = False, 
     fp32 arithmetic, one rounding.  Returns ``(q_out, k_out)``, new tensors or
     the ones passed (``q`` / ``k`` themselves rotate in place)."""
     _on_gpu("q", q)
-    _require(q.dtype in _ROT_DTYPES, lambda: f"rope: dtype {q.dtype} not in fp16 / bf16 / fp32", TypeError)
-    dev, dtype = q.device, q.dtype
-    _require(q.dim() == 3, lambda: f"q must be [tokens, heads, head_dim], got {tuple(q.shape)}")
+    dev, dtype, src_q, src_k = q.device, q.dtype, q, k
+    if not (dtype in _ROT_DTYPES and q.dim() == 3 and q.stride(2) == 1
+            and (k is None or (type(k) is torch.Tensor and k.dtype is dtype and k.device == dev and k.dim() == 3
+                               and k.shape[0] == q.shape[0] and k.stride(2) == 1))):
+        _require(dtype in _ROT_DTYPES, lambda: f"rope: dtype {dtype} not in fp16 / bf16 / fp32", TypeError)
+        _require(q.dim() == 3, lambda: f"q must be [tokens, heads, head_dim], got {tuple(q.shape)}")
+        src_q = _heads_view(q, "q", q.shape[0], dtype, dev)
+        src_k = None if k is None else _heads_view(k, "k", q.shape[0], dtype, dev)
     t, hq, d = q.shape
-    src_q, src_k = _heads_view(q, "q", t, dtype, dev), None
-    if k is not None:
-        src_k = _heads_view(k, "k", t, dtype, dev)
     args, keep = _rope_args(src_q, src_k, positions, cos_sin, sections, interleaved, pairing, q_norm, k_norm, eps)
     q_out = _rope_out(q_out, "q_out", q, dtype)
     if k is None:
@@ -1287,7 +1289,7 @@ def linear_attn_varlen(q, k, v, log_decay, state, cu_seqlens, max_seqlen, *, sta
     _require(max_seqlen >= 0, "max_seqlen must be >= 0")
     q, k, v, args, keep = _linear_args(q, k, v, log_decay, state, state_slots, reset, b)
     t, hq, d = q.shape
-    out = torch.empty((t, hq, d), dtype=q.dtype, device=q.device)
+    out = q.new_empty((t, hq, d))
     if b == 0:
         return out.zero_()
     lib = _lib.load()
@@ -1308,7 +1310,7 @@ def linear_attn_decode(q, k, v, log_decay, state, *, state_slots=None, reset=Non
     b = q.shape[0] if q.dim() else 0
     q, k, v, args, keep = _linear_args(q, k, v, log_decay, state, state_slots, reset, b)
     hq, d = q.shape[1:]
-    out = torch.empty((b, hq, d), dtype=q.dtype, device=q.device)
+    out = q.new_empty((b, hq, d))
     if b == 0:
         return out
     rc = _launch(q.device, _lib.load().s8kv_linear_attn_decode, q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(),
