@@ -579,11 +579,11 @@ int s8kv_append_rope_k8v3(const void* q, int num_q_heads, int64_t q_stride_t, in
  * outputs that depend on it non-finite, and no other.
  *
  * _varlen: sequence b's tokens are [cu_seqlens[b], cu_seqlens[b + 1]) (device
- * int32 [batch + 1]); max_seqlen only sizes the launch.  Rows of out behind
- * the last sequence are zeros.  workspace: s8kv_linear_attn_workspace_size
- * bytes (16-byte aligned, no initialisation) let long sequences be split
- * across workgroups; NULL or a smaller one runs unsplit.  Calls that overlap
- * on one workspace race.
+ * int32 [batch + 1], non-decreasing); max_seqlen only sizes the launch.  Rows
+ * of out outside all sequences are zeros.  workspace:
+ * s8kv_linear_attn_workspace_size bytes (16-byte aligned, no initialisation)
+ * let long sequences be split across workgroups; NULL or a smaller one runs
+ * unsplit.  Calls that overlap on one workspace race.
  * _decode: one token per sequence.
  */
 int64_t s8kv_linear_attn_workspace_size(int batch, int num_q_heads, int head_dim, int64_t num_tokens, int max_seqlen);

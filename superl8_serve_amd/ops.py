@@ -1281,7 +1281,7 @@ def linear_attn_varlen(q, k, v, log_decay, state, cu_seqlens, max_seqlen, *, sta
     ``[B]``, default b; distinct) and leaves its state there; a slot outside
     the pool marks a padding row (zeros out, no state).  ``reset`` (bool
     ``[B]``): True starts from an empty state.  Returns ``[T, Hq, D]`` of q's
-    dtype; rows behind the last sequence are zeros."""
+    dtype; rows outside all sequences are zeros."""
     _on_gpu("q", q)
     _on_gpu("cu_seqlens", cu_seqlens, torch.int32, q.device)
     _require(cu_seqlens.dim() == 1 and cu_seqlens.numel() >= 1, "cu_seqlens must be [B + 1]")

@@ -281,6 +281,125 @@ def test_captured_replays_and_two_streams():
     assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+def test_rows_outside_all_sequences():
+    rng = np.random.default_rng(51)
+    for n in (3, 90):  # the recurrence and the chunks
+        q, k, v = (inputs(rng, 2 * n + 20, 2, 64, torch.float16).to(DEV) for _ in range(3))
+        cu = np.array([7, 7 + n, 7 + n, 7 + 2 * n], np.int32)
+        g, state = t(slopes(2)), torch.zeros(3, 2, 64, 64, device=DEV)
+        out = ops.linear_attn_varlen(q, k, v, g, state, t(cu), n, scale=0.1)
+        cut = [x[7:7 + 2 * n] for x in (q, k, v)]
+        other = torch.zeros_like(state)
+        want = ops.linear_attn_varlen(*cut, g, other, t(cu - 7), n, scale=0.1)
+        assert not out[:7].any() and not out[7 + 2 * n:].any()
+        assert torch.equal(out[7:7 + 2 * n], want) and torch.equal(state, other)
+
+
+@pytest.mark.parametrize("name", list(DTYPES))
+@pytest.mark.parametrize("d", [32, 64, 256])
+def test_rows_without_alignment(d, name):
+    """Rows that 16-byte loads cannot take."""
+    rng = np.random.default_rng(d + 3)
+    dtype, lens, hq, hkv = DTYPES[name], [130, 1, 40], 4, 2
+    n, cu, g = sum(lens), np.array([0, 130, 131, 171], np.int32), slopes(4)
+    wide = [inputs(rng, n, h, d + 2, dtype).to(DEV) for h in (hq, hkv, hkv)]
+    q, k, v = (x[:, :, 1:-1] for x in wide)
+    state = rng.standard_normal((3, hq, d, d)).astype(np.float32)
+    pool = t(state)
+    got = ops.linear_attn_varlen(q, k, v, t(g), pool, t(cu), 130, scale=0.1).float().cpu().numpy()
+    step = pool.clone()
+    one = ops.linear_attn_decode(q[:3], k[:3], v[:3], t(g), step, scale=0.1).float().cpu().numpy()
+    q, k, v = (x.cpu() for x in (q, k, v))
+    for i in range(3):
+        at = slice(cu[i], cu[i + 1])
+        wo, ws, ro, rs = expect(q[at], k[at], v[at], g, state[i], 0.1, name)
+        check(f"out {i}", got[at], wo, ro, dtype)
+        check(f"state {i}", to_np(pool[i]), ws, rs)
+        wo, ws, ro, rs = expect(q[i:i + 1], k[i:i + 1], v[i:i + 1], g, to_np(pool[i]), 0.1, name)
+        check(f"step {i}", one[i:i + 1], wo, ro, dtype)
+        check(f"stepped state {i}", to_np(step[i]), ws, rs)
+
+
+@pytest.mark.parametrize("name", list(DTYPES))
+@pytest.mark.parametrize("d", [32, 256])
+def test_split_among_short_ones(d, name):
+    """Sequences that are split next to short, empty and padding ones."""
+    rng = np.random.default_rng(d + 11)
+    lens = [30, 0, 1100, 1, 64, 900, 0, 5]
+    run(rng, lens, 2, 1, d, name, slots=[4, 5, 0, 9, 1, -1, 2, 3], extra_rows=3)
+    run(rng, [700, 65], 2, 2, d, name, reset=[True, False], views=True)
+
+
+@pytest.mark.parametrize("name", list(DTYPES))
+def test_workspace_is_optional(name):
+    """The C entry without a workspace, and with one that is too small, runs unsplit."""
+    from superl8_serve_amd import _lib
+
+    lib, rng, n, d = _lib.load(), np.random.default_rng(61), 1500, 64
+    q, k, v = (inputs(rng, n, 2, d, DTYPES[name]) for _ in range(3))
+    dev, g, cu = [x.to(DEV) for x in (q, k, v)], t(slopes(2)), t(np.array([0, n], np.int32))
+    need = lib.s8kv_linear_attn_workspace_size(1, 2, d, n, n)
+    assert need > 0
+    wo, ws, ro, rs = expect(q, k, v, slopes(2), np.zeros((2, d, d)), 0.1, name)
+    work = torch.full((need,), 255, dtype=torch.uint8, device=DEV)  # (NaN: what is not written is not read)
+    for given, size in ((None, 0), (work, 16), (work, need)):
+        state, out = torch.zeros(1, 2, d, d, device=DEV), torch.empty(n, 2, d, dtype=DTYPES[name], device=DEV)
+        rc = lib.s8kv_linear_attn_varlen(
+            *(a for x in dev for a in (x.data_ptr(), x.stride(0), x.stride(1))), n, 2, 2, d, list(DTYPES).index(name),
+            g.data_ptr(), state.data_ptr(), 2 * d * d, 1, None, None, cu.data_ptr(), 1, n, 0.1, out.data_ptr(), 2 * d,
+            d, None if given is None else given.data_ptr(), size, torch.cuda.current_stream().cuda_stream)
+        assert rc == 0
+        check(f"workspace of {size}", out.float().cpu().numpy(), wo, ro, DTYPES[name])
+        check(f"state, workspace of {size}", to_np(state[0]), ws, rs)
+
+
+@pytest.mark.parametrize("hint", [500, 3000])
+@pytest.mark.parametrize("name", list(DTYPES))
+@pytest.mark.parametrize("what", ["v", "k", "state"])
+def test_non_finite_values_stay(what, name, hint):
+    """A NaN or infinity early on is in every later output that depends on it,
+    across segments and whatever the decay; the other columns (of its wave
+    too) stay right over many chunks."""
+    rng = np.random.default_rng(71)
+    n, d = 3000, 64
+    q, k, v = (inputs(rng, n, 2, d, DTYPES[name]) for _ in range(3))
+    for g in (np.array([-3.0, -1e-4], np.float32), np.array([-1e-4, 0.0], np.float32)):
+        wo, ws, ro, rs = expect(q, k, v, g, np.ones((2, d, d)), 0.1, name)
+        keep = np.ones((2, d), bool)
+        keep[:, 9] = False
+        for bad in (float("nan"), float("inf")):
+            x = {"q": q.to(DEV), "k": k.to(DEV), "v": v.to(DEV)}
+            state = torch.ones(1, 2, d, d, device=DEV)
+            if what == "state":
+                state[0, :, 5, 9] = bad
+            else:
+                x[what][70, :, 9] = bad
+            cu = t(np.array([0, n], np.int32))
+            got = ops.linear_attn_varlen(x["q"], x["k"], x["v"], t(g), state, cu, hint, scale=0.1).float().cpu().numpy()
+            new = to_np(state[0])
+            assert not np.isfinite(got[71:, :, 9]).any() and not np.isfinite(new[:, 5 if what == "state" else 9, 9]).any()
+            if what == "k":
+                assert not np.isfinite(new[:, 9]).any()
+                continue
+            check("other columns", got[:, keep], wo[:, keep], ro[:, keep], DTYPES[name])
+            check("other columns of the state", new.swapaxes(1, 2)[keep], ws.swapaxes(1, 2)[keep], rs.swapaxes(1, 2)[keep])
+
+
+@pytest.mark.parametrize("name", list(DTYPES))
+def test_columns_of_different_sizes(name):
+    """Value columns from 2^-12 to 2^6 next to each other, every one to its own size."""
+    rng = np.random.default_rng(81)
+    n, d = 300, 64
+    q, k = (inputs(rng, n, 2, d, DTYPES[name]) for _ in range(2))
+    size = np.exp2(np.arange(d) % 19 - 12).astype(np.float32)
+    v = torch.from_numpy(rng.uniform(1, 2, (n, 2, d)).astype(np.float32) * size).to(DTYPES[name])
+    state = torch.zeros(1, 2, d, d, device=DEV)
+    got = ops.linear_attn_varlen(q.to(DEV), k.to(DEV), v.to(DEV), t(slopes(2)), state, t(np.array([0, n], np.int32)), n, scale=0.1)
+    wo, ws, ro, rs = expect(q, k, v, slopes(2), np.zeros((2, d, d)), 0.1, name)
+    check("out", got.float().cpu().numpy(), wo, ro, DTYPES[name])
+    check("state", to_np(state[0]), ws, rs)
+
+
 def test_refusals():
     n, hq, hkv, d = 6, 4, 2, 64
     q, k, v = (torch.zeros(n, h, d, dtype=torch.float16, device=DEV) for h in (hq, hkv, hkv))
