@@ -408,6 +408,33 @@ class PagedKVCache:
             ops.quantize_kv_write_paged(k.contiguous(), v.contiguous(), self.k_cache[row], self.k_scale[row],
                                         self.v_cache[row], self.v_scale[row], slot_mapping)
 
+    def write_varlen_rope(self, layer: int, slot_mapping: torch.Tensor, q: torch.Tensor, k: torch.Tensor,
+                          v: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor, **rope) -> torch.Tensor:
+        """``write_prefill_varlen`` with the rotary positions (and q / k norms)
+        applied on the way, in one launch: ``q`` ``[T, Hq, D]``, ``k``, ``v``
+        ``[T, Hkv, D]`` as the projections leave them, fp16 or bf16.  Returns
+        the rotated q in fp16.  ``rope``: ``ops.rope``'s keywords, and ``k_out``
+        for the rotated k (the prefill attention over fresh keys)."""
+        row = self._layer_row(layer)
+        if self.v_quant == "lloydmax3":
+            return ops.quantize_kv_write_paged_k8v3_rope(
+                q, k, v, positions, cos_sin, self.k_cache[row], self.k_scale[row], self.v_packed[row],
+                self.v_norm[row], self.v_codebook[row], slot_mapping, self.lloyd_block, **rope)
+        return ops.quantize_kv_write_paged_rope(q, k, v, positions, cos_sin, self.k_cache[row], self.k_scale[row],
+                                                self.v_cache[row], self.v_scale[row], slot_mapping, **rope)
+
+    def write_decode_rope(self, layer: int, slots: list[int], positions: list[int], q: torch.Tensor,
+                          k_new: torch.Tensor, v_new: torch.Tensor, cos_sin: torch.Tensor, *,
+                          rope_positions: torch.Tensor | None = None, **rope) -> torch.Tensor:
+        """``write_decode`` with the rotation on the way: one token per sequence
+        at ``positions[i]`` of its slot, which is its rotary position too unless
+        ``rope_positions`` gives others (several axes).  Returns the rotated q
+        ``[B, Hq, D]``, what ``decode_attn`` takes."""
+        if rope_positions is None:
+            rope_positions = torch.tensor(positions, dtype=torch.int32, device=self.device)
+        return self.write_varlen_rope(layer, self.slot_mapping_for(slots, positions), q, k_new, v_new, rope_positions,
+                                      cos_sin, **rope)
+
     def write_prefill(self, layer: int, k: torch.Tensor, v: torch.Tensor, *, slot: int, start: int = 0,
                       positions: torch.Tensor | None = None) -> None:
         """k, v: fp16 ``[1, Hkv, S, D]``.  Positions ``[0, S)`` (or `positions`),

@@ -23,8 +23,12 @@ of gqa_attention.py:174-190, the multi-query verify
 (``attn_paged_verify[_k8v3]``) for the S decode launches of
 gqa_attention.py:217-314, the sliding-window decode
 (``attn_paged_decode_window[_k8v3]``) for gqa_attention.py:191-196, the fused
-K8V3 append (``quantize_kv_write_paged_k8v3``) for kv_cache.py:587-626 and the
-block copy (``copy_blocks``) behind copy-on-write and compaction.
+K8V3 append (``quantize_kv_write_paged_k8v3``) for kv_cache.py:587-626, the
+appends with the rotary positions applied on the way
+(``quantize_kv_write_paged[_k8v3]_rope``), linear attention with a decay per
+head for the other layers of hybrid models (``linear_attn_varlen``,
+``linear_attn_decode``) and the block copy (``copy_blocks``) behind
+copy-on-write and compaction.
 """
 
 from __future__ import annotations
@@ -45,8 +49,12 @@ from ..ops import (
     attn_paged_verify,
     attn_paged_verify_k8v3,
     copy_blocks,
+    linear_attn_decode,
+    linear_attn_varlen,
     quantize_kv_write_paged,
     quantize_kv_write_paged_k8v3,
+    quantize_kv_write_paged_k8v3_rope,
+    quantize_kv_write_paged_rope,
 )
 from . import quant
 
@@ -69,6 +77,10 @@ __all__ = [
     "attn_paged_verify",
     "attn_paged_verify_k8v3",
     "quantize_kv_write_paged_k8v3",
+    "quantize_kv_write_paged_rope",
+    "quantize_kv_write_paged_k8v3_rope",
+    "linear_attn_varlen",
+    "linear_attn_decode",
     "copy_blocks",
 ]
 
