@@ -186,9 +186,9 @@ static int launch(const Args& a, int head_dim, const char* what, hipStream_t str
 //
 // Operands of the 16-bit MFMAs that are fp32 values -- the decayed scores, S,
 // and the decayed v of the update -- go in as two halves, hi + lo (fp16
-// within 2^-22, bf16 within 2^-18 of the value), so that the state keeps fp32
-// grade and the output's only visible rounding is its last one; q, k and v
-// themselves are exact.  fp16 halves only reach from 2^-24 to 65504: scores,
+// within 2^-22, bf16 within 2^-18 of the value; the update's bf16 v in three,
+// 2^-26), so that the state keeps fp32 grade and the output's only visible
+// rounding is its last one; q, k and v themselves are exact.  fp16 halves only reach from 2^-24 to 65504: scores,
 // state and values are scaled by powers of two that bring their largest value
 // below 2^15 (the scores': of a row of a tile; S's: of a wave's columns; v's,
 // and with it the scale that S is kept at: of the chunk, changed only when a
@@ -238,6 +238,15 @@ __device__ __forceinline__ void split2(float a, float fa, float b, float fb, uin
   hi = pack2<DT>(a * fa, b * fb);
   asm("" : "+v"(hi));  // (the remainder reads hi as it was packed)
   lo = pack2<DT>(__builtin_fmaf(a, fa, -first<DT>(hi)), __builtin_fmaf(b, fb, -second<DT>(hi)));
+}
+// The same in three: what a bf16 pair leaves (2^-18) would be the state's error.
+__device__ __forceinline__ void split3(float a, float fa, float b, float fb, uint32_t& hi, uint32_t& mid, uint32_t& lo) {
+  hi = pack2<1>(a * fa, b * fb);
+  asm("" : "+v"(hi));
+  const float ra = __builtin_fmaf(a, fa, -first<1>(hi)), rb = __builtin_fmaf(b, fb, -second<1>(hi));
+  mid = pack2<1>(ra, rb);
+  asm("" : "+v"(mid));
+  lo = pack2<1>(ra - first<1>(mid), rb - second<1>(mid));
 }
 __device__ __forceinline__ uint32_t pk_max(uint32_t a, uint32_t b) {
   return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2_t, a), __builtin_bit_cast(u16x2_t, b)));
@@ -601,17 +610,25 @@ __global__ __launch_bounds__(2 * D, 2) void chunk_kernel(Args a) {
         for (int r = 0; r < 16; ++r) S[mt][r] = __builtin_fmaf(S[mt][r], drift, S[mt][r]);
     }
     constexpr int KB = KT < 2 ? KT : 2, KN = KT / KB, N = T * KN;  // key tiles a batch of reads, batches a step, batches
-    u32x4_t kf[2][KB], vh[2], vl[2];
+    constexpr int VN = DT == 0 ? 2 : 3;
+    u32x4_t kf[2][KB], vp[VN][2];
     auto decayed = [&](int t) {
       const float4_t* w = reinterpret_cast<const float4_t*>(left + 16 * t + 8 * g);
       const float4_t w0 = w[0], w1 = w[1];
 #pragma unroll
       for (int p = 0; p < 4; ++p) {
+        const float v0 = first<DT>(vf[t][p]), v1 = second<DT>(vf[t][p]);
+        const float f0 = p < 2 ? w0[2 * p] : w1[2 * p - 4], f1 = p < 2 ? w0[2 * p + 1] : w1[2 * p - 3];
         uint32_t x, y;
-        split2<DT>(first<DT>(vf[t][p]), p < 2 ? w0[2 * p] : w1[2 * p - 4], second<DT>(vf[t][p]),
-                   p < 2 ? w0[2 * p + 1] : w1[2 * p - 3], x, y);
-        vh[t % 2][p] = x;
-        vl[t % 2][p] = y;
+        if constexpr (DT == 0) {
+          split2<DT>(v0, f0, v1, f1, x, y);
+        } else {
+          uint32_t z;
+          split3(v0, f0, v1, f1, x, y, z);
+          vp[2][t % 2][p] = z;
+        }
+        vp[0][t % 2][p] = x;
+        vp[1][t % 2][p] = y;
       }
     };
 #pragma unroll
@@ -637,12 +654,12 @@ __global__ __launch_bounds__(2 * D, 2) void chunk_kernel(Args a) {
           if (q * N / 4 == n) exchanged(P, my_it, my_jt, q);
       }
 #pragma unroll
-      for (int m = 0; m < KB; ++m) S[m0 + m] = mfma<DT>(kf[n % 2][m], vh[t % 2], S[m0 + m]);
+      for (int i = 0; i < VN; ++i)
 #pragma unroll
-      for (int m = 0; m < KB; ++m) S[m0 + m] = mfma<DT>(kf[n % 2][m], vl[t % 2], S[m0 + m]);
+        for (int m = 0; m < KB; ++m) S[m0 + m] = mfma<DT>(kf[n % 2][m], vp[i][t % 2], S[m0 + m]);
       __builtin_amdgcn_sched_group_barrier(0x100, 2 * KB + 4, 0);
 #pragma unroll
-      for (int m = 0; m < 2 * KB; ++m) {
+      for (int m = 0; m < VN * KB; ++m) {
         __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
         __builtin_amdgcn_sched_group_barrier(0x002, 8, 0);
         __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);

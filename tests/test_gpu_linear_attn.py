@@ -400,6 +400,23 @@ def test_columns_of_different_sizes(name):
     check("state", to_np(state[0]), ws, rs)
 
 
+def test_slots_past_32_bits():
+    """A pool of more than 2^31 elements: slots at its end."""
+    hq, d = 32, 256
+    slots = 2 ** 31 // (hq * d * d) + 3
+    pool = torch.empty(slots, hq, d, d, device=DEV)
+    small = torch.randn(2, hq, d, d, device=DEV)
+    pool[slots - 2:] = small
+    at = t(np.array([slots - 1, slots - 2], np.int32))
+    rng = np.random.default_rng(91)
+    q, k, v = (inputs(rng, 90, hq, d, torch.bfloat16).to(DEV) for _ in range(3))
+    g, cu = t(slopes(hq)), t(np.array([0, 70, 90], np.int32))
+    for call in (lambda s, i: ops.linear_attn_varlen(q, k, v, g, s, cu, 70, state_slots=i, scale=0.1),
+                 lambda s, i: ops.linear_attn_decode(q[:2], k[:2], v[:2], g, s, state_slots=i, scale=0.1)):
+        want = call(small, t(np.array([1, 0], np.int32)))
+        assert torch.equal(call(pool, at), want) and torch.equal(pool[slots - 2:], small)
+
+
 def test_refusals():
     n, hq, hkv, d = 6, 4, 2, 64
     q, k, v = (torch.zeros(n, h, d, dtype=torch.float16, device=DEV) for h in (hq, hkv, hkv))

@@ -200,6 +200,37 @@ def test_write_equals_rope_then_append(kind):
 
 
 @pytest.mark.parametrize("kind", ["int8", "k8v3"])
+def test_write_past_32_bits(kind):
+    """A cache of more than 2^32 bytes: the rows at its end are the append's."""
+    hkv, d, bs = 8, 128, 16
+    blocks = 2 ** 32 // (hkv * d * bs) + 4
+    rng = np.random.default_rng(99)
+    q, k, v = (torch.from_numpy(rng.standard_normal((3, h, d)).astype(np.float16)).to(DEV) for h in (16, hkv, hkv))
+    pos, table = t(np.array([0, 5, 70], np.int32)), t(L.cos_sin_table(128, d))
+    cb = t(np.sort(rng.standard_normal(8)).astype(np.float32))
+
+    def cache(n):
+        e = lambda dtype, *last: torch.empty(n, hkv, bs, *last, dtype=dtype, device=DEV)  # noqa: E731
+        if kind == "int8":
+            return [e(torch.int8, d), e(torch.float32), e(torch.int8, d), e(torch.float32)]
+        return [e(torch.int8, d), e(torch.float32), e(torch.int32, 12), e(torch.float32, 1), cb]
+
+    small, large = cache(4), cache(blocks)
+    at = np.array([63, 0, 17], np.int32)
+    rq, rk = ops.rope(q, k, pos, table)
+    if kind == "int8":
+        ops.quantize_kv_write_paged(rk, v, *small, t(at))
+        got = ops.quantize_kv_write_paged_rope(q, k, v, pos, table, *large, t(at + (blocks - 4) * bs))
+    else:
+        ops.quantize_kv_write_paged_k8v3(rk, v, *small, t(at), 128)
+        got = ops.quantize_kv_write_paged_k8v3_rope(q, k, v, pos, table, *large, t(at + (blocks - 4) * bs), 128)
+    assert torch.equal(got, rq)
+    for a, b in zip(small[:4], large[:4]):
+        for s in at:
+            assert torch.equal(a[s // bs, :, s % bs], b[blocks - 4 + s // bs, :, s % bs])
+
+
+@pytest.mark.parametrize("kind", ["int8", "k8v3"])
 @pytest.mark.parametrize("shift", [0, 3])
 def test_write_non_finite_rows_stay_apart(kind, shift):
     """Infinities and NaN in one token's rows reach that token's outputs alone
