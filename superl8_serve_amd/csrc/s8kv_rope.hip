@@ -321,8 +321,17 @@ __device__ __forceinline__ bool cache_row(const Args& a, int64_t t, int h, uint6
 
 // modes: 0 q and k out, 1 int8 cache, 2 K8V3 cache.  A wave takes the heads of
 // its token (or tokens, where there are fewer heads than rows a wave) in
-// iterations of RPW rows, q's first, then k's, then v's, with the next
-// iteration's row in flight: its lanes' angles are fetched once.
+// iterations of RPW rows, q's first, then k's, then v's, with the next two
+// iterations' rows in flight: its lanes' angles are fetched once.  Waves that
+// share a token take its iterations in turn, so that each has rows of all three
+// kinds (a 3-bit V row takes several times a q row's instructions: 24.8 us for
+// 4,099 tokens of 28 + 4 heads, 25.3 in runs).
+// What bounds it is memory, and its latency where the tokens are few: 7,001
+// tokens of 32 + 8 bf16 heads of 128 with three axes 27 us (147 MB: 5.4 TB/s,
+// partly from the memory-side cache); 12,289 of 16 + 4 fp16 heads of 256, a
+// quarter rotated, 43 us (255 MB); with the int8 write, 16,384 tokens of 32 + 8
+// normalised heads, 83 us (379 MB, 4.6 TB/s); one token 4 us, of which an empty
+// launch takes 3.6.
 template <int D, int DT, int MODE>
 __global__ __launch_bounds__(64 * kWaves) void rope_rows_kernel(Args a) {
   using L = RowsLayout<D>;
@@ -332,8 +341,7 @@ __global__ __launch_bounds__(64 * kWaves) void rope_rows_kernel(Args a) {
   const int chunks = (a.iters + a.per_wave - 1) / a.per_wave;
   const int64_t wave = (int64_t)blockIdx.x * kWaves + wv;
   const int64_t group = wave / chunks;
-  const int it0 = (int)(wave - group * chunks) * a.per_wave;
-  const int it1 = min(a.iters, it0 + a.per_wave);
+  const int it0 = (int)(wave - group * chunks), it1 = a.iters;  // every chunks-th iteration: q, k and v rows for each
   const int hpi = 1 << a.hpi_log2, tokens = L::RPW >> a.hpi_log2;
   const int64_t t = group * tokens + (L::row(lane) >> a.hpi_log2);
   const int sub = L::row(lane) & (hpi - 1);
@@ -374,7 +382,7 @@ __global__ __launch_bounds__(64 * kWaves) void rope_rows_kernel(Args a) {
   };
   Raw<DT> next{}, after{};  // the rows of the next iteration, and of the one after it
   if (it0 < it1) next = fetch(it0);
-  if (it0 + 1 < it1) after = fetch(it0 + 1);
+  if (it0 + chunks < it1) after = fetch(it0 + chunks);
   Angles<D> angles;
   if (it0 < nq + nk) {
     Angles<D>::gather(a, group * tokens, tokens, lane, lds[wv]);
@@ -382,13 +390,13 @@ __global__ __launch_bounds__(64 * kWaves) void rope_rows_kernel(Args a) {
   }
 
 #pragma unroll 1
-  for (int it = it0; it < it1; ++it) {
+  for (int it = it0; it < it1; it += chunks) {
     const int kind = kind_of(it), h = first_head(it, kind) + sub;
     const bool live = here && h < (kind == 0 ? a.q.heads : a.k.heads);
     float x[16];
     expand<DT>(next, x);
     next = after;
-    if (it + 2 < it1) after = fetch(it + 2);
+    if (it + 2 * chunks < it1) after = fetch(it + 2 * chunks);
     if (kind < 2) {
       if (kind == 0 ? a.q.norm : a.k.norm) normalise<D>(a, norms[kind] + 16 * li, x);
       angles.turn(a, x);
