@@ -1054,16 +1054,19 @@ def _rope_args(q, k, positions, cos_sin, sections, interleaved, pairing, q_norm,
     the checks one by one take twice an op's other host time.)"""
     dev = q.get_device()
     t, _, d = q.shape
-    if not (type(positions) is type(cos_sin) is torch.Tensor and positions.get_device() == cos_sin.get_device() == dev
-            and positions.dtype is torch.int32 and cos_sin.dtype is torch.float32 and sections is None
-            and not interleaved and positions.shape == (t,) and positions.is_contiguous() and cos_sin.dim() == 2
-            and cos_sin.is_contiguous() and cos_sin.shape[0] > 0 and 0 < cos_sin.shape[1] <= d
-            and cos_sin.shape[1] % 2 == 0 and pairing in _PAIRINGS and (k is None or k.shape[2] == d)
-            and type(q_norm) is type(k_norm) and _norm_ok(q_norm, d, dev) and _norm_ok(k_norm, d, dev)
-            and (q_norm is None or q_norm.dtype is k_norm.dtype)):
+    usual = (type(positions) is type(cos_sin) is torch.Tensor and positions.get_device() == cos_sin.get_device() == dev
+             and positions.dtype is torch.int32 and cos_sin.dtype is torch.float32 and sections is None
+             and not interleaved and positions.shape == (t,) and positions.is_contiguous() and cos_sin.dim() == 2
+             and cos_sin.is_contiguous() and pairing in _PAIRINGS and (k is None or k.shape[2] == d))
+    if usual:
+        rows, rot = cos_sin.shape
+        usual = (rows > 0 and 0 < rot <= d and rot % 2 == 0 and type(q_norm) is type(k_norm)
+                 and (q_norm is None or (_norm_ok(q_norm, d, dev) and _norm_ok(k_norm, d, dev)
+                                         and q_norm.dtype is k_norm.dtype)))
+    if not usual:
         positions, cos_sin, q_norm, k_norm = _rope_checked(q, k, positions, cos_sin, sections, interleaved, pairing,
                                                            q_norm, k_norm)
-    rows, rot = cos_sin.shape
+        rows, rot = cos_sin.shape
     if sections is None:
         axes, amap = 1, None
     else:
@@ -1077,7 +1080,7 @@ def _rope_args(q, k, positions, cos_sin, sections, interleaved, pairing, q_norm,
 
 def _rope_out(out, name: str, like: torch.Tensor, dtype) -> torch.Tensor:
     if out is None:
-        return like.new_empty(like.shape, dtype=dtype)
+        return like.new_empty(like.shape) if dtype is like.dtype else like.new_empty(like.shape, dtype=dtype)
     _on_gpu(name, out, dtype, like.device)
     _require(out.shape == like.shape and out.stride(2) == 1,
              lambda: f"{name} must be {tuple(like.shape)} with a unit stride on its last dim")
@@ -1102,14 +1105,15 @@ def rope(q, k, positions, cos_sin, *, sections=None, interleaved: bool = False, 
     fp32 arithmetic, one rounding.  Returns ``(q_out, k_out)``, new tensors or
     the ones passed (``q`` / ``k`` themselves rotate in place)."""
     _on_gpu("q", q)
-    dev, dtype, src_q, src_k = q.device, q.dtype, q, k
-    if not (dtype in _ROT_DTYPES and q.dim() == 3 and q.stride(2) == 1
+    dev, dtype, src_q, src_k, qs = q.device, q.dtype, q, k, q.stride()
+    if not (dtype in _ROT_DTYPES and len(qs) == 3 and qs[2] == 1
             and (k is None or (type(k) is torch.Tensor and k.dtype is dtype and k.device == dev and k.dim() == 3
                                and k.shape[0] == q.shape[0] and k.stride(2) == 1))):
         _require(dtype in _ROT_DTYPES, lambda: f"rope: dtype {dtype} not in fp16 / bf16 / fp32", TypeError)
         _require(q.dim() == 3, lambda: f"q must be [tokens, heads, head_dim], got {tuple(q.shape)}")
         src_q = _heads_view(q, "q", q.shape[0], dtype, dev)
         src_k = None if k is None else _heads_view(k, "k", q.shape[0], dtype, dev)
+        qs = src_q.stride()
     t, hq, d = q.shape
     args, keep = _rope_args(src_q, src_k, positions, cos_sin, sections, interleaved, pairing, q_norm, k_norm, eps)
     q_out = _rope_out(q_out, "q_out", q, dtype)
@@ -1119,11 +1123,13 @@ def rope(q, k, positions, cos_sin, *, sections=None, interleaved: bool = False, 
         kos = (None, 0, 0)
     else:
         k_out = _rope_out(k_out, "k_out", k, dtype)
-        ks = (src_k.data_ptr(), k.shape[1], src_k.stride(0), src_k.stride(1))
-        kos = (k_out.data_ptr(), k_out.stride(0), k_out.stride(1))
+        st, kos = src_k.stride(), k_out.stride()
+        ks = (src_k.data_ptr(), k.shape[1], st[0], st[1])
+        kos = (k_out.data_ptr(), kos[0], kos[1])
     if t:
-        rc = _launch(dev, _lib.load().s8kv_rope, src_q.data_ptr(), hq, src_q.stride(0), src_q.stride(1), *ks, t, d,
-                     _ROT_DTYPES[dtype], *args, q_out.data_ptr(), q_out.stride(0), q_out.stride(1), *kos, _stream(q))
+        qos = q_out.stride()
+        rc = _launch(dev, _lib.load().s8kv_rope, src_q.data_ptr(), hq, qs[0], qs[1], *ks, t, d, _ROT_DTYPES[dtype], *args,
+                     q_out.data_ptr(), qos[0], qos[1], *kos, _stream(q))
         _lib.check(rc, "rope")
     return q_out, k_out
 
@@ -1158,10 +1164,10 @@ def _rope_write(what, entry, q, k, v, positions, cos_sin, k_cache, k_scale, slot
         k_out = _rope_out(k_out, "k_out", k, torch.float16)
         kos = (k_out.data_ptr(), k_out.stride(0), k_out.stride(1))
     if t:
-        rc = _launch(dev, entry, q.data_ptr(), hq, q.stride(0), q.stride(1), k.data_ptr(), v.data_ptr(), hkv,
-                     k.stride(0), k.stride(1), v.stride(0), v.stride(1), t, d, _LINEAR_DTYPES[dtype], *args,
-                     q_out.data_ptr(), q_out.stride(0), q_out.stride(1), *kos, slot_mapping.data_ptr(),
-                     k_cache.data_ptr(), k_scale.data_ptr(), *tail, n, bs, _stream(q))
+        qs, ks, vs, qos = q.stride(), k.stride(), v.stride(), q_out.stride()
+        rc = _launch(dev, entry, q.data_ptr(), hq, qs[0], qs[1], k.data_ptr(), v.data_ptr(), hkv, ks[0], ks[1], vs[0],
+                     vs[1], t, d, _LINEAR_DTYPES[dtype], *args, q_out.data_ptr(), qos[0], qos[1], *kos,
+                     slot_mapping.data_ptr(), k_cache.data_ptr(), k_scale.data_ptr(), *tail, n, bs, _stream(q))
         _lib.check(rc, what)
     return q_out
 
@@ -1250,24 +1256,32 @@ def _linear_checked(q, k, v, log_decay, state, state_slots, reset, batch):
 
 
 def _linear_args(q, k, v, log_decay, state, state_slots, reset, batch):
-    """(q, k, v, the C arguments from the dtype on, what must outlive the
-    call).  The usual call is recognised by one test."""
-    dev, dtype = q.device, q.dtype
-    if not (type(log_decay) is type(state) is torch.Tensor and dtype in _LINEAR_DTYPES and k.dtype is v.dtype is dtype
-            and k.device == v.device == log_decay.device == state.device == dev
-            and log_decay.dtype is state.dtype is torch.float32 and q.dim() == k.dim() == 3 and k.shape == v.shape
-            and q.shape[0] == k.shape[0] and q.shape[2] == k.shape[2] and k.shape[1] > 0
-            and q.shape[1] % k.shape[1] == 0 and q.stride(2) == k.stride(2) == v.stride(2) == 1
-            and log_decay.shape == q.shape[1:2] and log_decay.is_contiguous() and state.dim() == 4
-            and state.is_contiguous() and state.shape[1:] == (q.shape[1], q.shape[2], q.shape[2]) and reset is None
-            and (state_slots is None or (state_slots.dtype is torch.int32 and state_slots.device == dev
-                                         and state_slots.shape == (batch,) and state_slots.is_contiguous()))):
+    """(the C arguments from q to reset, the output's shape, what must outlive
+    the call).  The usual call is recognised by one test."""
+    dtype, dev = q.dtype, q.get_device()
+    qs, ks = q.shape, k.shape
+    usual = len(qs) == len(ks) == 3 and reset is None and type(log_decay) is type(state) is torch.Tensor
+    if usual:
+        t, hq, d = qs
+        hkv, slots = ks[1], state.shape[0] if state.dim() else 0
+        usual = (k.dtype is v.dtype is dtype and dtype in _LINEAR_DTYPES
+                 and k.get_device() == v.get_device() == log_decay.get_device() == state.get_device() == dev
+                 and log_decay.dtype is state.dtype is torch.float32 and ks == v.shape and ks[0] == t and ks[2] == d
+                 and hkv > 0 and hq % hkv == 0 and log_decay.shape == (hq,) and log_decay.is_contiguous()
+                 and state.shape == (slots, hq, d, d) and state.is_contiguous()
+                 and (state_slots is None or (state_slots.dtype is torch.int32 and state_slots.get_device() == dev
+                                              and state_slots.shape == (batch,) and state_slots.is_contiguous())))
+    qt, kt, vt = q.stride(), k.stride(), v.stride()
+    if not (usual and qt[2] == kt[2] == vt[2] == 1):
         q, k, v, log_decay, state_slots, reset = _linear_checked(q, k, v, log_decay, state, state_slots, reset, batch)
-    _, hq, d = q.shape
-    slots = state.shape[0]
-    args = (_LINEAR_DTYPES[dtype], log_decay.data_ptr(), state.data_ptr(), state.stride(0) if slots > 1 else hq * d * d,
-            slots, None if state_slots is None else state_slots.data_ptr(), None if reset is None else reset.data_ptr())
-    return q, k, v, args, (log_decay, state_slots, reset)
+        t, hq, d = qs = q.shape
+        hkv, slots = k.shape[1], state.shape[0]
+        qt, kt, vt = q.stride(), k.stride(), v.stride()
+    args = (q.data_ptr(), qt[0], qt[1], k.data_ptr(), kt[0], kt[1], v.data_ptr(), vt[0], vt[1], t, hq, hkv, d,
+            _LINEAR_DTYPES[dtype], log_decay.data_ptr(), state.data_ptr(),
+            state.stride(0) if slots > 1 else hq * d * d, slots,
+            None if state_slots is None else state_slots.data_ptr(), None if reset is None else reset.data_ptr())
+    return args, qs, (q, k, v, log_decay, state_slots, reset)
 
 
 def linear_attn_varlen(q, k, v, log_decay, state, cu_seqlens, max_seqlen, *, state_slots=None, reset=None, scale):
@@ -1287,17 +1301,16 @@ def linear_attn_varlen(q, k, v, log_decay, state, cu_seqlens, max_seqlen, *, sta
     _require(cu_seqlens.dim() == 1 and cu_seqlens.numel() >= 1, "cu_seqlens must be [B + 1]")
     cu_seqlens, b, max_seqlen = cu_seqlens.contiguous(), cu_seqlens.numel() - 1, int(max_seqlen)
     _require(max_seqlen >= 0, "max_seqlen must be >= 0")
-    q, k, v, args, keep = _linear_args(q, k, v, log_decay, state, state_slots, reset, b)
-    t, hq, d = q.shape
-    out = q.new_empty((t, hq, d))
+    args, shape, keep = _linear_args(q, k, v, log_decay, state, state_slots, reset, b)
+    t, hq, d = shape
+    out = q.new_empty(shape)
     if b == 0:
         return out.zero_()
     lib = _lib.load()
     ws_bytes = int(lib.s8kv_linear_attn_workspace_size(b, hq, d, t, max_seqlen))
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
-    rc = _launch(q.device, lib.s8kv_linear_attn_varlen, q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0),
-                 k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), t, hq, k.shape[1], d, *args,
-                 cu_seqlens.data_ptr(), b, max_seqlen, scale, out.data_ptr(), hq * d, d,
+    rc = _launch(q.device, lib.s8kv_linear_attn_varlen, *args, cu_seqlens.data_ptr(), b, max_seqlen, scale,
+                 out.data_ptr(), hq * d, d,
                  None if ws is None else ws.data_ptr(), ws_bytes, _stream(q))
     _lib.check(rc, "linear_attn_varlen")
     return out
@@ -1308,13 +1321,12 @@ def linear_attn_decode(q, k, v, log_decay, state, *, state_slots=None, reset=Non
     ``k``, ``v`` ``[B, Hkv, D]``; returns ``[B, Hq, D]``."""
     _on_gpu("q", q)
     b = q.shape[0] if q.dim() else 0
-    q, k, v, args, keep = _linear_args(q, k, v, log_decay, state, state_slots, reset, b)
-    hq, d = q.shape[1:]
-    out = q.new_empty((b, hq, d))
+    args, shape, keep = _linear_args(q, k, v, log_decay, state, state_slots, reset, b)
+    out = q.new_empty(shape)
     if b == 0:
         return out
-    rc = _launch(q.device, _lib.load().s8kv_linear_attn_decode, q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(),
-                 k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), b, hq, k.shape[1], d, *args,
-                 scale, out.data_ptr(), hq * d, d, _stream(q))
+    _, hq, d = shape
+    # (the batch is the token count of the shared arguments)
+    rc = _launch(q.device, _lib.load().s8kv_linear_attn_decode, *args, scale, out.data_ptr(), hq * d, d, _stream(q))
     _lib.check(rc, "linear_attn_decode")
     return out
