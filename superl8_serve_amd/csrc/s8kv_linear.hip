@@ -305,7 +305,7 @@ __global__ __launch_bounds__(2 * D, 2) void chunk_kernel(Args a) {
   constexpr int NW = D / 32, NT = 64 * NW, KT = D / 32;
   constexpr int C = kChunk<D>, IT = C / 32, T = C / 16;  // its 32-token tiles and 16-token steps
   constexpr int QP = 2 * D + 16, KP = 2 * D + 32, PP = 2 * C + 16;  // row pitches that spread a read's rows over the banks
-  constexpr int PH = IT == 1 ? 64 * PP : C * PP;  // bytes of the scores' hi halves (and of lo; with one tile, room for a second)
+  constexpr int PH = C * PP;  // bytes of the scores' hi halves (and of lo)
   constexpr int KO = OUT ? C * QP : 0, VO = KO + C * KP, PO = VO + C * KP, EO = PO + (OUT ? 2 * PH : 0);
   constexpr int MO = EO + (OUT ? 4 * 32 * 4 : 0);  // (EO: the score rows' exponents by tile; MO: the waves' largest |v|)
   constexpr int LO = MO + (4 * NW + 15) / 16 * 16 + 128;  // 32 ones, lambda^0 .. lambda^C, then 2^-sv lambda^(C - 1) .. lambda^0
@@ -418,8 +418,9 @@ __global__ __launch_bounds__(2 * D, 2) void chunk_kernel(Args a) {
   int sv = 0;  // S is kept times 2^-sv, which brings v's largest value near 2^13 (fp16)
   bool first_chunk = true;
   // the wave's score tile: (0, 0), (1, 1) and (1, 0) by wave; waves without one make one that is not read
-  const int my_at = IT == 1 ? (wv == 0 ? 0 : 3) : (NW == 2 ? 2 * wv : (wv < 3 ? wv : 3));
-  const int my_it = IT == 1 ? (wv == 0 ? 0 : 1) : (my_at == 1 || my_at == 2), my_jt = IT == 1 ? 0 : (my_at == 1 || my_at == 3);
+  constexpr bool TURNS = IT == 2;  // (a chunk of one tile: its scores are the first wave's, ahead of the others' work)
+  const int my_at = NW == 2 ? 2 * wv : (wv < 3 ? wv : 3);
+  const int my_it = my_at == 1 || my_at == 2, my_jt = my_at == 1 || my_at == 3;
   // (vmcnt 0: with the state's loads still counted as outstanding at the loop's head, the compiler waits for the
   // loop's own loads where it overwrites registers that held the state's)
   __builtin_amdgcn_s_waitcnt(0x0F70);
@@ -545,7 +546,7 @@ __global__ __launch_bounds__(2 * D, 2) void chunk_kernel(Args a) {
       *reinterpret_cast<u32x2_t*>(to + PH) = u32x2_t{l0, l1};
     };
     if constexpr (OUT) {
-      if constexpr (NW < 3 && IT == 2) {  // the tiles that the waves have no turn for below
+      if constexpr (!TURNS || NW < 3) {  // the tiles that the waves have no turn for below
         auto tile = [&](int it, int jt, int at) {
           float16_t acc = {};
 #pragma unroll
@@ -554,8 +555,12 @@ __global__ __launch_bounds__(2 * D, 2) void chunk_kernel(Args a) {
 #pragma unroll
           for (int q = 0; q < 4; ++q) exchanged(acc, it, jt, q);
         };
-        if (wv == 0) tile(1, 1, 1);
-        if (NW == 1) tile(1, 0, 2);
+        if (!TURNS) {
+          if (wv == 0) tile(0, 0, 0);
+        } else {
+          if (wv == 0) tile(1, 1, 1);
+          if (NW == 1) tile(1, 0, 2);
+        }
       }
       // ---- o^T = S^T q^T (rows: value dims, columns: tokens), and the wave's score tile ----
       const float s_down = pow2(-es);
@@ -574,7 +579,7 @@ __global__ __launch_bounds__(2 * D, 2) void chunk_kernel(Args a) {
       u32x4_t kp[2];
 #pragma unroll
       for (int it = 0; it < IT; ++it) qf[0][it] = q8(it, 0);
-      kp[0] = k8(my_jt, 0);
+      if constexpr (TURNS) kp[0] = k8(my_jt, 0);
       halves(0);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -587,7 +592,7 @@ __global__ __launch_bounds__(2 * D, 2) void chunk_kernel(Args a) {
         if (s + 1 < 2 * KT) {
 #pragma unroll
           for (int it = 0; it < IT; ++it) qf[(s + 1) % 2][it] = q8(it, s + 1);
-          kp[(s + 1) % 2] = k8(my_jt, s + 1);
+          if constexpr (TURNS) kp[(s + 1) % 2] = k8(my_jt, s + 1);
           halves(s + 1);
         } else {
 #pragma unroll
@@ -598,11 +603,11 @@ __global__ __launch_bounds__(2 * D, 2) void chunk_kernel(Args a) {
         for (int it = 0; it < IT; ++it) O[it] = mfma<DT>(hi[s % 2], qf[s % 2][it], O[it]);
 #pragma unroll
         for (int it = 0; it < IT; ++it) O[it] = mfma<DT>(lo[s % 2], qf[s % 2][it], O[it]);
-        P = mfma<DT>(kp[s % 2], qp, P);
-        if (s + 1 < 2 * KT) __builtin_amdgcn_sched_group_barrier(0x100, IT + 2, 0);
+        if constexpr (TURNS) P = mfma<DT>(kp[s % 2], qp, P);
+        if (s + 1 < 2 * KT) __builtin_amdgcn_sched_group_barrier(0x100, TURNS ? IT + 2 : IT, 0);
         else __builtin_amdgcn_sched_group_barrier(0x100, 2 * T, 0);
 #pragma unroll
-        for (int n = 0; n < 2 * IT + 1; ++n) {
+        for (int n = 0; n < 2 * IT + TURNS; ++n) {
           __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
           __builtin_amdgcn_sched_group_barrier(0x002, IT == 2 ? 9 : 14, 0);
         }
@@ -647,7 +652,7 @@ __global__ __launch_bounds__(2 * D, 2) void chunk_kernel(Args a) {
 #pragma unroll
     for (int m = 0; m < KB; ++m) kf[0][m] = col8(KO, 0, 32 * m);
     decayed(0);
-    if constexpr (OUT) masked(P, my_it == my_jt, my_at);
+    if constexpr (OUT && TURNS) masked(P, my_it == my_jt, my_at);
     __builtin_amdgcn_sched_barrier(0);
     // (without a next chunk the descriptors are the present one's: the loads come to nothing, but their number is known)
 #pragma unroll
@@ -661,7 +666,7 @@ __global__ __launch_bounds__(2 * D, 2) void chunk_kernel(Args a) {
         for (int m = 0; m < KB; ++m) kf[(n + 1) % 2][m] = col8(KO, (n + 1) / KN, 32 * ((n + 1) % KN * KB + m));
         if ((n + 1) % KN == 0) decayed(t + 1);
       }
-      if constexpr (OUT) {
+      if constexpr (OUT && TURNS) {
 #pragma unroll
         for (int q = 0; q < 4; ++q)
           if (q * N / 4 == n) exchanged(P, my_it, my_jt, q);
