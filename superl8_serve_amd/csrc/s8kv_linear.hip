@@ -245,7 +245,8 @@ __device__ __forceinline__ float second(uint32_t w) {
 // a fa, b fb as 16-bit pairs hi + lo; lo takes the exact remainder.  (fp16:
 // v_fma_mixlo / mixhi would make each half in one instruction, but their
 // partial writes cost wait states: the whole chunk 5.0 us instead of 5.2 this
-// way, head_dim 128 with one workgroup a CU.)
+// way, head_dim 128 with one workgroup a CU.  bf16: a dot product with (-1, 0)
+// instead of the unpacking and the subtraction was 3 % slower.)
 template <int DT>
 __device__ __forceinline__ void split2(float a, float fa, float b, float fb, uint32_t& hi, uint32_t& lo) {
   hi = pack2<DT>(a * fa, b * fb);
@@ -424,8 +425,8 @@ __global__ __launch_bounds__(2 * D, 2) void chunk_kernel(Args a) {
   // (vmcnt 0: with the state's loads still counted as outstanding at the loop's head, the compiler waits for the
   // loop's own loads where it overwrites registers that held the state's)
   __builtin_amdgcn_s_waitcnt(0x0F70);
-  // A bound of the wave's finite |S|: the largest at first, then the largest
-  // that a chunk's halves had, decayed, and what the chunk can have added.
+  // A bound of the wave's finite |S|: the largest at first, then decayed and
+  // raised by what each chunk can have added.
   auto largest = [&]() {
     uint32_t m = 0;
 #pragma unroll
@@ -511,7 +512,6 @@ __global__ __launch_bounds__(2 * D, 2) void chunk_kernel(Args a) {
     u32x4_t vf[T];  // the wave's columns of v, 8 tokens a lane
     float16_t O[IT] = {}, P = {};
     const int es = DT == 0 ? excess(s_bound, -100) : 0;
-    uint32_t hi_max = 0;
     const float lambda_n = pw[len];
     float down = 1.0f;
     // A tile of the scores (rows j: key tokens, columns i), done in three
@@ -572,7 +572,6 @@ __global__ __launch_bounds__(2 * D, 2) void chunk_kernel(Args a) {
           split2<DT>(S[s / 2][8 * (s % 2) + 2 * p], s_down, S[s / 2][8 * (s % 2) + 2 * p + 1], s_down, x, y);
           hi[s % 2][p] = x;
           lo[s % 2][p] = y;
-          if constexpr (DT == 0) hi_max = pk_max(hi_max, x & 0x7FFF7FFFu);
         }
       };
       // one step's reads and halves ahead, and S's decay behind, in the shadow of the step's MFMAs
@@ -711,10 +710,8 @@ __global__ __launch_bounds__(2 * D, 2) void chunk_kernel(Args a) {
           for (int it = t / 2; it < IT; ++it) O[it] = mfma<DT>(vf[t], p8(half, it, t), O[it]);
       }
       if constexpr (DT == 0) {
-        hi_max = wave_pk_max(pk_max(hi_max, hi_max >> 16));
-        const uint32_t m = (uint32_t)uniform((int)hi_max) & 0xFFFFu;
-        if (m < 0x7C00u) s_bound = magnitude(m) * pow2(es) * lambda_n + kv_max * pow2(-sv);
-        else s_bound = largest();  // (a column is infinite or NaN: the others keep their own size)
+        // (every 16 chunks the largest itself: the bound only grows in between, and what it has too much of costs bits)
+        s_bound = applied ? s_bound * lambda_n + kv_max * pow2(-sv) : largest();
       }
 #pragma unroll
       for (int it = 0; it < IT; ++it) {
