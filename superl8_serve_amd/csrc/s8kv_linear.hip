@@ -788,12 +788,21 @@ static int launch_chunks(Args& a, const char* what, hipStream_t stream) {
 // side, so a batch is even enough while its longest sequence is no longer than
 // the tokens a CU has to do altogether; else segments of half of those, two a
 // CU.  Splitting reads k and v of all but the last segments a second time.
-constexpr int kLeastSegment = 256;
+// Where a CU has few tokens to do, a segment's chain of chunks and the scan over
+// the segments' D x D states share the time, so segments grow with the root of
+// length x D; past 256 tokens the chain weighs more.  (One sequence, us, with
+// 128 / 256 tokens a segment and unsplit: 512 tokens x 32 heads of 128 30.2 / 35.5 /
+// 34.1, of 64 21.6 / 29.0 / 31.0; 2,048 tokens of 128 51.5 / 45.5 / 119; with
+// several sequences the CUs are full at more: 2 x 1,024 of 128, 192 tokens a
+// segment 50.6, 256 44.4.  Less than two and a half segments do not pay: 300
+// tokens of 128 26.1 split, 23.7 not; 384 26.9 / 27.3, of 64 20.2 / 24.3.)
 static int segment_tokens(int64_t tokens, int heads, int head_dim, int max_seqlen) {
   if (max_seqlen > tokens) max_seqlen = (int)tokens;  // (a graph's bucket, say)
   const int64_t share = tokens * heads * head_dim / (128 * (int64_t)device_cus());
-  if (max_seqlen <= share + share / 5 || max_seqlen <= 2 * kLeastSegment) return 0;
-  const int64_t seg = share / 2 > kLeastSegment ? share / 2 : kLeastSegment;
+  int64_t least = 128;
+  while (least < 256 && (3 * least < 4 * share || 4 * least * least < (int64_t)max_seqlen * head_dim)) least += 64;
+  if (max_seqlen <= share + share / 5 || 2 * (int64_t)max_seqlen <= 5 * least) return 0;
+  const int64_t seg = share / 2 > least ? share / 2 : least;
   const int64_t n = (max_seqlen + seg - 1) / seg;
   return (int)((max_seqlen + n - 1) / n + 63) / 64 * 64;
 }
