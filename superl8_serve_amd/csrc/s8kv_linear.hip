@@ -808,9 +808,10 @@ static int segment_tokens(int64_t tokens, int heads, int head_dim, int max_seqle
 }
 template <int DT>
 static int launch_varlen(Args& a, int head_dim, int max_seqlen, const char* what, hipStream_t stream) {
-  // (a chunk's rows have 32-bit offsets, one bit of them for the rows that are not there)
-  auto rows = [](const void* p, int64_t t, int64_t h) {
-    return (uintptr_t)p % 16 == 0 && t % 8 == 0 && h % 8 == 0 && t >= 0 && t < (1 << 24);
+  // (a chunk's rows have 32-bit offsets, one bit of them for the rows that are not there: rows that share bytes with
+  // the next, broadcast tokens say, would find themselves there)
+  auto rows = [head_dim](const void* p, int64_t t, int64_t h) {
+    return (uintptr_t)p % 16 == 0 && t % 8 == 0 && h % 8 == 0 && t >= head_dim && t < (1 << 24);
   };
   if (!(rows(a.q, a.q_t, a.q_h) && rows(a.k, a.k_t, a.k_h) && rows(a.v, a.v_t, a.v_h) && rows(a.out, a.o_t, a.o_h)))
     return launch<DT>(a, head_dim, what, stream);

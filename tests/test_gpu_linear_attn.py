@@ -320,6 +320,26 @@ def test_rows_without_alignment(d, name):
         check(f"stepped state {i}", to_np(step[i]), ws, rs)
 
 
+@pytest.mark.parametrize("hint", [0, 5000])
+@pytest.mark.parametrize("what", ["broadcast", "windows"])
+def test_rows_that_share_bytes(what, hint):
+    """One token's rows for all tokens (stride 0), and rows that overlap the next."""
+    rng = np.random.default_rng(13)
+    n, hq, d, g = 75, 2, 64, slopes(2)
+    if what == "broadcast":
+        k, v = (inputs(rng, 1, hq, d, torch.float16).to(DEV).expand(n, hq, d) for _ in range(2))
+    else:
+        k, v = (inputs(rng, 1, 1, 8 * n + hq * d, torch.float16).to(DEV).as_strided((n, hq, d), (8, d, 1)) for _ in range(2))
+    q, state = inputs(rng, n, hq, d, torch.float16), torch.zeros(2, hq, d, d, device=DEV)
+    cu = np.array([0, 70, 75], np.int32)
+    got = ops.linear_attn_varlen(q.to(DEV), k, v, t(g), state, t(cu), hint, scale=0.1).float().cpu().numpy()
+    for b in range(2):
+        at = slice(cu[b], cu[b + 1])
+        wo, ws, ro, rs = expect(q[at], k.cpu()[at], v.cpu()[at], g, np.zeros((hq, d, d)), 0.1, "fp16")
+        check(f"out {b}", got[at], wo, ro, torch.float16)
+        check(f"state {b}", to_np(state[b]), ws, rs)
+
+
 @pytest.mark.parametrize("name", list(DTYPES))
 @pytest.mark.parametrize("d", [32, 256])
 def test_split_among_short_ones(d, name):
