@@ -417,7 +417,6 @@ __global__ __launch_bounds__(2 * D, 2) void chunk_kernel(Args a) {
   };
 
   int sv = 0;  // S is kept times 2^-sv, which brings v's largest value near 2^13 (fp16)
-  bool first_chunk = true;
   // the wave's score tile: (0, 0), (1, 1) and (1, 0) by wave; waves without one make one that is not read
   constexpr bool TURNS = IT == 2;  // (a chunk of one tile: its scores are the first wave's, ahead of the others' work)
   const int my_at = NW == 2 ? 2 * wv : (wv < 3 ? wv : 3);
@@ -492,13 +491,12 @@ __global__ __launch_bounds__(2 * D, 2) void chunk_kernel(Args a) {
       }
       if constexpr (DT == 0) {
         const float vmax = magnitude(m), now_v = vmax * pow2(-sv);
-        if (first_chunk || (vmax > 0.0f && (now_v < 512.0f || now_v >= 32768.0f))) {
+        if (vmax > 0.0f && (now_v < 512.0f || now_v >= 32768.0f)) {
           const int now = excess(vmax, -100) + 1;
 #pragma unroll
           for (int mt = 0; mt < KT; ++mt) S[mt] = S[mt] * pow2(sv) * pow2(-now);
           s_bound = s_bound * pow2(sv) * pow2(-now);
           sv = now;
-          first_chunk = false;
           for (int n = tid; n < C; n += NT) left[n] = pw[C - 1 - n] * pow2(-sv);
           __syncthreads();
         }

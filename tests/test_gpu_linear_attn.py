@@ -130,6 +130,26 @@ def test_sizes_of_values(size):
     run(rng, [200, 33], 2, 2, 128, "bf16", size=size, scale=0.005 / size ** 2)
 
 
+@pytest.mark.parametrize("name", list(DTYPES))
+@pytest.mark.parametrize("n", [70, 1000])
+def test_nothing_but_the_state(n, name):
+    """Values of zero (at first, or all of them) and of the smallest size next to a large state."""
+    rng = np.random.default_rng(n)
+    d, g = 64, slopes(2)
+    q, k, v = (inputs(rng, n, 2, d, DTYPES[name]) for _ in range(3))
+    for zero, small in ((64, 1.0), (n, 1.0), (5, 2.0 ** -20)):
+        x = v * small
+        x[:zero] = 0
+        s0 = (rng.standard_normal((2, d, d)) * 2.0 ** 60).astype(np.float32)
+        state = t(s0[None])
+        cu = t(np.array([0, n], np.int32))
+        scale = 2.0 ** -62
+        got = ops.linear_attn_varlen(q.to(DEV), k.to(DEV), x.to(DEV), t(g), state, cu, n, scale=scale).float().cpu().numpy()
+        wo, ws, ro, rs = expect(q, k, x, g, s0, scale, name)
+        check("out", got, wo, ro, DTYPES[name])
+        check("state", to_np(state[0]), ws, rs)
+
+
 def test_unset_max_seqlen_is_only_a_hint():
     rng = np.random.default_rng(3)
     q, k, v = (inputs(rng, 400, 2, 64, torch.float16).to(DEV) for _ in range(3))
