@@ -247,9 +247,11 @@ __device__ __forceinline__ float second(uint32_t w) {
 // partial writes cost wait states: the whole chunk 5.0 us instead of 5.2 this
 // way, head_dim 128 with one workgroup a CU.  bf16: a dot product with (-1, 0)
 // instead of the unpacking and the subtraction was 3 % slower.)
-template <int DT>
+// PACKED: a and b come out of packed halves; fp16's multiply-add takes them there.
+template <int DT, bool PACKED = false>
 __device__ __forceinline__ void split2(float a, float fa, float b, float fb, uint32_t& hi, uint32_t& lo) {
-  hi = pack2<DT>(a * fa, b * fb);
+  if constexpr (DT == 0 && PACKED) hi = pack2<DT>(__builtin_fmaf(a, fa, 0.0f), __builtin_fmaf(b, fb, 0.0f));
+  else hi = pack2<DT>(a * fa, b * fb);
   asm("" : "+v"(hi));  // (the remainder reads hi as it was packed)
   lo = pack2<DT>(__builtin_fmaf(a, fa, -first<DT>(hi)), __builtin_fmaf(b, fb, -second<DT>(hi)));
 }
@@ -636,7 +638,7 @@ __global__ __launch_bounds__(2 * D, 2) void chunk_kernel(Args a) {
         const float f0 = p < 2 ? w0[2 * p] : w1[2 * p - 4], f1 = p < 2 ? w0[2 * p + 1] : w1[2 * p - 3];
         uint32_t x, y;
         if constexpr (DT == 0) {
-          split2<DT>(v0, f0, v1, f1, x, y);
+          split2<DT, true>(v0, f0, v1, f1, x, y);
         } else {
           uint32_t z;
           split3(v0, f0, v1, f1, x, y, z);
