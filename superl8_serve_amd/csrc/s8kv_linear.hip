@@ -202,11 +202,11 @@ static int launch(const Args& a, int head_dim, const char* what, hipStream_t str
 // neighbour there starts to lose bits: the halves end at 2^-25.
 //
 // What bounds it (32 heads of 128, 1.05 M (token, head) pairs): the output pass
-// takes 258 us, 4.2 TB/s of q, k, v and out with the matrix cores 37 % busy, and
-// 227 us when every row comes from the L2: memory, and the chain of a chunk
-// (products, exchange, two barriers) with two workgroups a CU to overlap, weigh
-// the same.  16-column waves (twice the waves, S's halves made from half the
-// columns): 10 % slower.
+// takes 254 us, 4.2 TB/s of q, k, v and out with the matrix cores 38 % busy, and
+// 221 us when every row comes from the L2: memory and the vector instructions
+// (820 a wave and chunk, most of them splits into halves) weigh the same; of 256,
+// with chunks half as long, the instructions alone take 780 us of 850.
+// 16-column waves (twice the waves, half the splits each): 10 % slower.
 //
 // A masked score is zero, but zero times an infinite or NaN v of a later
 // token is not: a chunk whose v is not finite is redone token by token.
