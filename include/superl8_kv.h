@@ -576,7 +576,8 @@ int s8kv_append_rope_k8v3(const void* q, int num_q_heads, int64_t q_stride_t, in
  * written.  reset uint8 [batch] or NULL: a non-zero entry starts its sequence
  * from an empty state (the slot's old contents are not read), so a sequence
  * of no tokens leaves zeros there.  A non-finite state or input makes the
- * outputs that depend on it non-finite, and no other.
+ * outputs that depend on it non-finite, and no other.  With fp16 inputs a
+ * state's magnitude must stay below 2^64 (products are scaled by powers of two).
  *
  * _varlen: sequence b's tokens are [cu_seqlens[b], cu_seqlens[b + 1]) (device
  * int32 [batch + 1], non-decreasing); max_seqlen only sizes the launch.  Rows

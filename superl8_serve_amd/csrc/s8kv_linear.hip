@@ -199,7 +199,9 @@ static int launch(const Args& a, int head_dim, const char* what, hipStream_t str
 // below 2^15 (the scores': of a row of a tile; S's: of a wave's columns; v's,
 // and with it the scale that S is kept at: of the chunk, changed only when a
 // chunk's leaves [2^9, 2^15]).  What is 2^19 times smaller than its largest
-// neighbour there starts to lose bits: the halves end at 2^-25.
+// neighbour there starts to lose bits: the halves end at 2^-25.  (States stay
+// below 2^64: their scale goes up by 2^37 under the least v, their products
+// with q by 2^32 where a row's scores are zero.)
 //
 // What bounds it (32 heads of 128, 1.05 M (token, head) pairs): the output pass
 // takes 254 us, 4.2 TB/s of q, k, v and out with the matrix cores 38 % busy, and
