@@ -1294,8 +1294,9 @@ def linear_attn_varlen(q, k, v, log_decay, state, cu_seqlens, max_seqlen, *, sta
     updated in place: sequence b continues from slot ``state_slots[b]`` (int32
     ``[B]``, default b; distinct) and leaves its state there; a slot outside
     the pool marks a padding row (zeros out, no state).  ``reset`` (bool
-    ``[B]``): True starts from an empty state.  Returns ``[T, Hq, D]`` of q's
-    dtype; rows outside all sequences are zeros."""
+    ``[B]``): True starts from an empty state.  ``max_seqlen`` sizes the launch
+    (longer sequences are done all the same).  fp16: states stay below 2^64.
+    Returns ``[T, Hq, D]`` of q's dtype; rows outside all sequences are zeros."""
     _on_gpu("q", q)
     _on_gpu("cu_seqlens", cu_seqlens, torch.int32, q.device)
     _require(cu_seqlens.dim() == 1 and cu_seqlens.numel() >= 1, "cu_seqlens must be [B + 1]")
