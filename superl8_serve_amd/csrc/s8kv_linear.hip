@@ -188,7 +188,8 @@ static int launch(const Args& a, int head_dim, const char* what, hipStream_t str
 // chunk's loads are in flight meanwhile.  The C x C scores are made by up to
 // three waves, one 32 x 32 tile on or below the diagonal each, and exchanged
 // through LDS.  C is 64; 32 at head_dim 256, whose columns of S take 128
-// registers a lane.
+// registers a lane, at head_dim 32, whose single wave makes the scores alone,
+// and for short sequences.
 //
 // Operands of the 16-bit MFMAs that are fp32 values -- the decayed scores, S,
 // and the decayed v of the update -- go in as two halves, hi + lo (fp16
@@ -220,7 +221,7 @@ typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
 typedef float float16_t __attribute__((ext_vector_type(16)));
 
 template <int D>
-constexpr int kChunk = D == 256 ? 32 : 64;
+constexpr int kChunk = D == 64 || D == 128 ? 64 : 32;
 
 template <int DT>
 __device__ __forceinline__ float16_t mfma(u32x4_t a, u32x4_t b, float16_t c) {
@@ -305,10 +306,10 @@ __device__ __forceinline__ int64_t part_of(const Args& a, int b, int first) { re
 // state, from zero, for scan_kernel; of all its tokens, also those whose decay
 // rounds to zero, since an infinite or NaN one has to arrive (leaving them out
 // saved 3 % at 16,384 tokens, 32 heads of 128).
-template <int D, int DT, bool OUT>
+template <int D, int DT, bool OUT, int C = kChunk<D>>
 __global__ __launch_bounds__(2 * D, 2) void chunk_kernel(Args a) {
   constexpr int NW = D / 32, NT = 64 * NW, KT = D / 32;
-  constexpr int C = kChunk<D>, IT = C / 32, T = C / 16;  // its 32-token tiles and 16-token steps
+  constexpr int IT = C / 32, T = C / 16;  // its 32-token tiles and 16-token steps
   constexpr int QP = 2 * D + 16, KP = 2 * D + 32, PP = 2 * C + 16;  // row pitches that spread a read's rows over the banks
   constexpr int PH = C * PP;  // bytes of the scores' hi halves (and of lo)
   constexpr int KO = OUT ? C * QP : 0, VO = KO + C * KP, PO = VO + C * KP, EO = PO + (OUT ? 2 * PH : 0);
@@ -548,7 +549,7 @@ __global__ __launch_bounds__(2 * D, 2) void chunk_kernel(Args a) {
       *reinterpret_cast<u32x2_t*>(to + PH) = u32x2_t{l0, l1};
     };
     if constexpr (OUT) {
-      if constexpr (!TURNS || NW < 3) {  // the tiles that the waves have no turn for below
+      if constexpr (!TURNS || NW < 3) {  // the tile that no wave has a turn for below
         auto tile = [&](int it, int jt, int at) {
           float16_t acc = {};
 #pragma unroll
@@ -557,12 +558,7 @@ __global__ __launch_bounds__(2 * D, 2) void chunk_kernel(Args a) {
 #pragma unroll
           for (int q = 0; q < 4; ++q) exchanged(acc, it, jt, q);
         };
-        if (!TURNS) {
-          if (wv == 0) tile(0, 0, 0);
-        } else {
-          if (wv == 0) tile(1, 1, 1);
-          if (NW == 1) tile(1, 0, 2);
-        }
+        if (wv == 0) tile(TURNS, TURNS, TURNS);
       }
       // ---- o^T = S^T q^T (rows: value dims, columns: tokens), and the wave's score tile ----
       const float s_down = pow2(-es);
@@ -773,7 +769,7 @@ __global__ __launch_bounds__(256) void scan_kernel(Args a) {
 }
 
 template <int D, int DT>
-static int launch_chunks(Args& a, const char* what, hipStream_t stream) {
+static int launch_chunks(Args& a, int max_seqlen, const char* what, hipStream_t stream) {
   const int64_t pairs = (int64_t)a.batch * a.heads, grid = pairs * a.num_seg;
   S8KV_REQUIRE(grid < (int64_t(1) << 31) && pairs * (D * D / 1024) < (int64_t(1) << 31), S8KV_ERR_INVALID,
                "%s: too many (sequence, head) pairs", what);
@@ -781,7 +777,13 @@ static int launch_chunks(Args& a, const char* what, hipStream_t stream) {
     hipLaunchKernelGGL((chunk_kernel<D, DT, false>), dim3((unsigned)grid), dim3(2 * D), 0, stream, a);
     hipLaunchKernelGGL((scan_kernel<D>), dim3((unsigned)(pairs * (D * D / 1024))), dim3(256), 0, stream, a);
   }
-  hipLaunchKernelGGL((chunk_kernel<D, DT, true>), dim3((unsigned)grid), dim3(2 * D), 0, stream, a);
+  // chunks of 32 for sequences that fill no more (32 sequences x 32 heads of 64, 16 tokens: 10.1 us, 17.3 with 64; of 128
+  // 29.2 / 30.6); of 64 also for short ones in numbers, since more of their workgroups fit a CU's LDS (64 sequences x 32
+  // heads: 40 tokens 26.1 / 32.3, 130 tokens 42.2 / 58.3, 250 tokens 85.0 / 84.6; four sequences of 100 12.2 / 11.3)
+  if (kChunk<D> > 32 && (max_seqlen <= 32 || (D == 64 && max_seqlen <= 192 && pairs >= 2 * device_cus())))
+    hipLaunchKernelGGL((chunk_kernel<D, DT, true, 32>), dim3((unsigned)grid), dim3(2 * D), 0, stream, a);
+  else
+    hipLaunchKernelGGL((chunk_kernel<D, DT, true>), dim3((unsigned)grid), dim3(2 * D), 0, stream, a);
   return check_launch(what);
 }
 
@@ -817,14 +819,15 @@ static int launch_varlen(Args& a, int head_dim, int max_seqlen, const char* what
   };
   if (!(rows(a.q, a.q_t, a.q_h) && rows(a.k, a.k_t, a.k_h) && rows(a.v, a.v_t, a.v_h) && rows(a.out, a.o_t, a.o_h)))
     return launch<DT>(a, head_dim, what, stream);
-  // a few tokens: the recurrence reads and writes the state at once (head_dim 128, 32 sequences x 32 heads: 6 tokens
-  // 27.7 us against the chunk's 34.2, 8 tokens 32.0 / 33.9, 12 tokens 39.5 / 34.2; head_dim 64: 12 tokens 15.7 / 18.5)
-  if ((int64_t)max_seqlen * head_dim <= 768) return launch<DT>(a, head_dim, what, stream);
+  // a few tokens: the recurrence reads and writes the state at once (recurrence / chunk, 32 sequences x 32 heads of 128:
+  // 5 tokens 26.8 / 27.8 us, 8 tokens 31.6 / 28.1; one sequence 6.3 / 7.9, 8.2 / 7.9; of 64: 5 tokens 10.1 / 10.0, 8
+  // tokens 12.8 / 10.1; of 256: 5 tokens 105 / 106, 8 tokens 120 / 106; of 32: 4 tokens 7.1 / 6.2, one sequence 4.8 / 5.2)
+  if (max_seqlen <= (head_dim == 32 ? 3 : 5)) return launch<DT>(a, head_dim, what, stream);
   switch (head_dim) {
-    case 32: return launch_chunks<32, DT>(a, what, stream);
-    case 64: return launch_chunks<64, DT>(a, what, stream);
-    case 128: return launch_chunks<128, DT>(a, what, stream);
-    case 256: return launch_chunks<256, DT>(a, what, stream);
+    case 32: return launch_chunks<32, DT>(a, max_seqlen, what, stream);
+    case 64: return launch_chunks<64, DT>(a, max_seqlen, what, stream);
+    case 128: return launch_chunks<128, DT>(a, max_seqlen, what, stream);
+    case 256: return launch_chunks<256, DT>(a, max_seqlen, what, stream);
   }
   return S8KV_ERR_UNSUPPORTED;
 }

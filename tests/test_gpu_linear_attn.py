@@ -92,6 +92,37 @@ def test_lengths(d, name):
 
 
 @pytest.mark.parametrize("name", list(DTYPES))
+@pytest.mark.parametrize("d", [32, 64, 128, 256])
+def test_short_sequences(d, name):
+    """No more than 32 tokens, whose chunks are half as long; few, which the recurrence takes."""
+    rng = np.random.default_rng(d + 1)
+    run(rng, [1, 32, 0, 7, 31, 17, 6, 5, 4, 3], 4, 2, d, name, extra_rows=2)
+    run(rng, [5, 1, 0, 4], 4, 4, d, name)
+    run(rng, [6, 2], 2, 1, d, name, views=True)
+
+
+@pytest.mark.parametrize("name", list(DTYPES))
+def test_short_sequences_in_numbers(name):
+    rng = np.random.default_rng(6)
+    run(rng, [int(n) for n in rng.integers(0, 140, 70)], 8, 4, 64, name)
+
+
+@pytest.mark.parametrize("name", list(DTYPES))
+@pytest.mark.parametrize("d", [64, 128])
+def test_hint_of_32_for_longer_sequences(d, name):
+    rng = np.random.default_rng(d + 2)
+    q, k, v = (inputs(rng, 200, 2, d, DTYPES[name]) for _ in range(3))
+    state = torch.zeros(2, 2, d, d, device=DEV)
+    cu = np.array([0, 150, 200], np.int32)
+    got = ops.linear_attn_varlen(q.to(DEV), k.to(DEV), v.to(DEV), t(slopes(2)), state, t(cu), 32, scale=0.1).float().cpu().numpy()
+    for b in range(2):
+        at = slice(cu[b], cu[b + 1])
+        wo, ws, ro, rs = expect(q[at], k[at], v[at], slopes(2), np.zeros((2, d, d)), 0.1, name)
+        check(f"out {b}", got[at], wo, ro, DTYPES[name])
+        check(f"state {b}", to_np(state[b]), ws, rs)
+
+
+@pytest.mark.parametrize("name", list(DTYPES))
 @pytest.mark.parametrize("hq,hkv,d", [(1, 1, 128), (6, 2, 64), (8, 1, 128), (5, 5, 32), (4, 2, 256)])
 def test_heads_views_and_tail(hq, hkv, d, name):
     rng = np.random.default_rng(hq + d)
