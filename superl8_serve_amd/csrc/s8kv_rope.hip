@@ -324,8 +324,8 @@ __device__ __forceinline__ bool cache_row(const Args& a, int64_t t, int h, uint6
 // iterations of RPW rows, q's first, then k's, then v's, with the next two
 // iterations' rows in flight: its lanes' angles are fetched once.  Waves that
 // share a token take its iterations in turn, so that each has rows of all three
-// kinds (a 3-bit V row takes several times a q row's instructions: 24.8 us for
-// 4,099 tokens of 28 + 4 heads, 25.3 in runs).
+// kinds (a 3-bit V row takes several times a q row's instructions: 2 % of the
+// 21.6 us that 4,099 tokens of 28 + 4 heads take).
 // What bounds it is memory, and its latency where the tokens are few: 7,001
 // tokens of 32 + 8 bf16 heads of 128 with three axes 27 us (147 MB: 5.4 TB/s,
 // partly from the memory-side cache); 12,289 of 16 + 4 fp16 heads of 256, a
@@ -556,9 +556,11 @@ static int launch(Args& a, const char* what, hipStream_t stream) {
     a.iters = (a.q.heads + hpi - 1) / hpi + (a.k.heads + hpi - 1) / hpi + (a.v.heads + hpi - 1) / hpi;
     const int64_t groups = (a.tokens + tokens - 1) / tokens;
     // as many waves as the GPU holds, each with an equal share of its tokens' iterations (a wave's start, the chain
-    // from the positions to the angles, takes as long as several of them)
+    // from the positions to the angles, takes as long as several of them); rounded up, since waves that wait for a place
+    // cost more than longer ones (4,099 tokens of 28 + 4 heads into K8V3 24.9 us rounded down, 21.6 up; 1,000 of 32 + 8
+    // int8 10.3 / 8.6)
     const int64_t want = (int64_t)device_cus() * 16;
-    const int64_t each = groups * a.iters / want;
+    const int64_t each = (groups * a.iters + want - 1) / want;
     const int parts = (int)(each < 1 ? a.iters : (each > a.iters ? 1 : (a.iters + each - 1) / each));
     a.per_wave = (a.iters + parts - 1) / parts;
     const int64_t waves = groups * ((a.iters + a.per_wave - 1) / a.per_wave);
