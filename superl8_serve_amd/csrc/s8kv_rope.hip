@@ -325,7 +325,7 @@ __device__ __forceinline__ bool cache_row(const Args& a, int64_t t, int h, uint6
 // iterations' rows in flight: its lanes' angles are fetched once.  Waves that
 // share a token take its iterations in turn, so that each has rows of all three
 // kinds (a 3-bit V row takes several times a q row's instructions: 2 % of the
-// 21.6 us that 4,099 tokens of 28 + 4 heads take).
+// 20.0 us that 4,099 tokens of 28 + 4 heads take).
 // What bounds it is memory, and its latency where the tokens are few: 7,001
 // tokens of 32 + 8 bf16 heads of 128 with three axes 27 us (147 MB: 5.4 TB/s,
 // partly from the memory-side cache); 12,289 of 16 + 4 fp16 heads of 256, a
@@ -555,13 +555,12 @@ static int launch(Args& a, const char* what, hipStream_t stream) {
     const int hpi = 1 << a.hpi_log2, tokens = RPW >> a.hpi_log2;
     a.iters = (a.q.heads + hpi - 1) / hpi + (a.k.heads + hpi - 1) / hpi + (a.v.heads + hpi - 1) / hpi;
     const int64_t groups = (a.tokens + tokens - 1) / tokens;
-    // as many waves as the GPU holds, each with an equal share of its tokens' iterations (a wave's start, the chain
-    // from the positions to the angles, takes as long as several of them); rounded up, since waves that wait for a place
-    // cost more than longer ones (4,099 tokens of 28 + 4 heads into K8V3 24.9 us rounded down, 21.6 up; 1,000 of 32 + 8
-    // int8 10.3 / 8.6)
-    const int64_t want = (int64_t)device_cus() * 16;
-    const int64_t each = (groups * a.iters + want - 1) / want;
-    const int parts = (int)(each < 1 ? a.iters : (each > a.iters ? 1 : (a.iters + each - 1) / each));
+    // as many waves as the GPU holds (16 a CU, 12 with the 3-bit search's registers), no more: a wave's start, the chain
+    // from the positions to the angles, takes as long as several iterations, and waves that wait for a place cost more
+    // than longer ones (4,099 tokens of 28 + 4 heads into K8V3 24.9 us with 1.5 times as many, 21.6 with 1.3, 20.0 so;
+    // 1,000 of 32 + 8 int8 10.3 / 8.6 / 8.6, 3,000 19.4 / 19.3 / 16.9)
+    const int64_t want = (int64_t)device_cus() * (MODE == 2 ? 12 : 16);
+    const int parts = (int)(want < groups ? 1 : (want / groups > a.iters ? a.iters : want / groups));
     a.per_wave = (a.iters + parts - 1) / parts;
     const int64_t waves = groups * ((a.iters + a.per_wave - 1) / a.per_wave);
     const int64_t grid = (waves + kWaves - 1) / kWaves;
